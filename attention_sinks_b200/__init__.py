@@ -7,13 +7,20 @@ Public API (src/sinkcache/__init__.py:1-7 of the reference):
     StreamRunner                            -- CUDA-graph streaming runner (both caches)
     flash_decode, register                  -- decode attention + Transformers backend
     apply_rope, rerotate                    -- RoPE helpers
+
+Operators beside the reference's:
+    rotary, rope_frequencies                -- rotation of q and k on the GPU, with its gradients
+    PagedKVCache                            -- paged cache: append with rotation, decode attention
+                                               over a shared prefix and each sequence's own rows
 """
 
 from .cache import SinkCache, SinkLayer, find_inv_freq
 from .cache_v2 import SinkCacheV2, SinkLayerV2
 from .decode_attention import decode_attention_forward, flash_decode, register
 from .graphs import StreamRunner
-from .rope import apply_rope, rerotate
+from .paged import PagedKVCache
+from .rope import apply_rope, rerotate, rope_frequencies, rotary
 
 __all__ = ["SinkCache", "SinkLayer", "SinkCacheV2", "SinkLayerV2", "StreamRunner", "find_inv_freq",
-           "flash_decode", "register", "decode_attention_forward", "apply_rope", "rerotate"]
+           "flash_decode", "register", "decode_attention_forward", "apply_rope", "rerotate",
+           "rotary", "rope_frequencies", "PagedKVCache"]

@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libsinkcache_b200.so")
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 OP_APPEND, OP_EVICT, OP_ATTEND, OP_FUSED_STEP = 0, 1, 2, 3
-STATUS_WAIT_TIMEOUT = 1
+STATUS_WAIT_TIMEOUT, STATUS_BAD_PAGE = 1, 2
 
 _DTYPE_CODE = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
@@ -25,7 +25,8 @@ EXPORTED_SYMBOLS = (
     "sink_evict_rerotate", "sink_decode_attention", "sink_fused_decode_step", "sink_read_status",
     "sink_decode_attention_noalloc", "sink_v2_place", "sink_v2_decode_step", "sink_prepare_device",
     "sink_debug_fail_next_wait", "sink_plan_launch", "sink_evict_rerotate_keycopy", "sink_v2_gather",
-    "sink_debug_cluster_capacity", "sink_launch_count",
+    "sink_debug_cluster_capacity", "sink_launch_count", "sink_rotary", "sink_paged_append",
+    "sink_paged_workspace_bytes", "sink_paged_attention",
 )
 LAUNCH_SPLIT, LAUNCH_CLUSTER, LAUNCH_TENSOR = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -54,6 +55,28 @@ class Rows(ctypes.Structure):
     ]
 
 
+class Rotation(ctypes.Structure):
+    """sink_rotation_t"""
+    _fields_ = [
+        ("inv_freq", ctypes.c_void_p), ("rot_half", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("inverse", ctypes.c_int32),
+    ]
+
+
+class PagedKV(ctypes.Structure):
+    """sink_paged_kv_t"""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p), ("status", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("pages", ctypes.c_int32),
+        ("table_width", ctypes.c_int32), ("pad_", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("k_stride_p", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v_stride_p", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -62,6 +85,7 @@ def _declare(lib):
     i32, i64, sz, vp, fp = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p
     pkv, prows = ctypes.POINTER(KVBuffers), ctypes.POINTER(Rows)
     pi32 = ctypes.POINTER(ctypes.c_int32)
+    ppaged, prot = ctypes.POINTER(PagedKV), ctypes.POINTER(Rotation)
     sig = {
         "sink_abi_version": (i32, []),
         "sink_launch_count": (ctypes.c_uint64, []),
@@ -82,6 +106,10 @@ def _declare(lib):
         "sink_decode_attention_noalloc": (i32, [prows, pkv, i32, ctypes.c_float, vp, i64, vp, i64, i64, vp]),
         "sink_v2_place": (i32, [pkv, prows, prows, prows, vp, i32, prows, vp, i64, i32, i32, vp, i32, vp]),
         "sink_v2_gather": (i32, [pkv, i32, i32, i32, i64, i64, prows, prows, prows, prows, vp]),
+        "sink_rotary": (i32, [i32, i32, prows, prows, prows, prows, vp, i64, prot, vp]),
+        "sink_paged_append": (i32, [ppaged, prows, prows, vp, prows, prows, prot, vp]),
+        "sink_paged_workspace_bytes": (sz, [i32] * 6),
+        "sink_paged_attention": (i32, [prows, ppaged, i32, ctypes.c_float, vp, i64, i64, vp, sz, vp]),
         "sink_v2_decode_step": (i32, [pkv, prows, prows, prows, vp, i32, vp, i32, i32, vp, i32, prows,
                                       ctypes.c_float, vp, i64, vp, i64, i64, vp, sz, vp]),
     }
@@ -457,3 +485,52 @@ def v2_gather(kbuf: torch.Tensor, vbuf: torch.Tensor, n_sink: int, window: int, 
                               ctypes.byref(rows_desc(out_k)), ctypes.byref(rows_desc(out_v)),
                               stream_handle(kbuf.device))
     _check(rc, "sink_v2_gather")
+
+
+# ------------------------------------------------- rotation, paged append, paged attention
+
+
+def raise_status(status: int) -> None:
+    """Raise what the status bits of a paged cache say."""
+    if status & STATUS_BAD_PAGE:
+        raise RuntimeError("sinkcache_b200: a position past the block table or a page index outside the pool was "
+                           "met since the last check; it was not accessed, and the results that needed it are void")
+    if status:
+        raise RuntimeError(f"sinkcache_b200 kernel status 0x{status:x}: a bounded wait ran out; the results of the "
+                           "launches since the last check are void")
+
+
+def rotary(q: torch.Tensor, q_out: torch.Tensor, k: torch.Tensor | None, k_out: torch.Tensor | None,
+           positions: torch.Tensor, rot: Rotation) -> None:
+    """q_out = rotate(q) and k_out = rotate(k), [B, H, T, D] each, at positions [T] or [B, T]."""
+    stride_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    rc = lib().sink_rotary(q.shape[0], q.shape[3], ctypes.byref(rows_desc(q)), ctypes.byref(rows_desc(q_out)),
+                           ctypes.byref(rows_desc(k)) if k is not None else None,
+                           ctypes.byref(rows_desc(k_out)) if k is not None else None,
+                           positions.data_ptr(), stride_b, ctypes.byref(rot), stream_handle(q.device))
+    _check(rc, "sink_rotary")
+
+
+def paged_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None,
+                 q: torch.Tensor | None, q_out: torch.Tensor | None, rot: Rotation | None) -> None:
+    """The first counts[b] tokens of k, v [B, Hkv, T, D] into their pages (k rotated), q beside them."""
+    rc = lib().sink_paged_append(ctypes.byref(kv), ctypes.byref(rows_desc(k)), ctypes.byref(rows_desc(v)),
+                                 counts.data_ptr() if counts is not None else None,
+                                 ctypes.byref(rows_desc(q)) if q is not None else None,
+                                 ctypes.byref(rows_desc(q_out)) if q is not None else None,
+                                 ctypes.byref(rot) if rot is not None else None, stream_handle(k.device))
+    _check(rc, "sink_paged_append")
+
+
+def paged_workspace_bytes(batch: int, heads_kv: int, heads_q: int, head_dim: int, shared_len: int,
+                          num_sms: int) -> int:
+    return int(lib().sink_paged_workspace_bytes(batch, heads_kv, heads_q, head_dim, shared_len, num_sms))
+
+
+def paged_attention(q: torch.Tensor, kv: PagedKV, shared_len: int, scale: float, out: torch.Tensor,
+                    workspace: torch.Tensor) -> None:
+    """out[B, 1, Hq, D] = attention of q [B, Hq, 1, D] over each sequence's rows [0, lens[b])."""
+    rc = lib().sink_paged_attention(ctypes.byref(rows_desc(q)), ctypes.byref(kv), shared_len, scale, out.data_ptr(),
+                                    out.stride(0), out.stride(2), workspace.data_ptr(), workspace.numel(),
+                                    stream_handle(q.device))
+    _check(rc, "sink_paged_attention")

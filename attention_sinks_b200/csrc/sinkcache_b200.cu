@@ -11,6 +11,7 @@
 
 #include "../../include/sinkcache_b200.h"
 #include "sink_attend_tc.cuh"
+#include "sink_host.h"
 #include "sink_kernels.cuh"
 #include "sink_v2.cuh"
 
@@ -256,6 +257,10 @@ int32_t make_plan(int32_t op, int32_t batch, int32_t heads_kv, int32_t heads_q, 
   return SINK_OK;
 }
 
+}  // namespace
+
+namespace sinkb200 {
+
 int device_sms(int* dev_out) {
   static std::atomic<int> cache[64];
   int dev = 0;
@@ -268,6 +273,10 @@ int device_sms(int* dev_out) {
   }
   return n;
 }
+
+}  // namespace sinkb200
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -300,10 +309,18 @@ int32_t check_rows(const sink_rows_t* r, int32_t dtype, int32_t batch, int32_t h
 // Kernel launches this library has issued in the process (sink_launch_count).
 std::atomic<uint64_t> g_launches{0};
 
+}  // namespace
+
+namespace sinkb200 {
+
 cudaError_t counted(cudaError_t err) {
   if (err == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
   return err;
 }
+
+}  // namespace sinkb200
+
+namespace {
 
 // Launch with programmatic stream serialization: the kernel may begin launching while its
 // predecessor in the stream finishes (every kernel here waits on the grid dependency before
@@ -585,6 +602,10 @@ int32_t plan_attention(const sink_rows_t* q, const sink_kv_buffers_t* kv, int32_
   return SINK_OK;
 }
 
+}  // namespace
+
+namespace sinkb200 {
+
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime.
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static std::atomic<void*> cached{nullptr};
@@ -599,6 +620,10 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   }
   return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
 }
+
+}  // namespace sinkb200
+
+namespace {
 
 // 4-D map over one cache buffer [B, Hkv, slots, 128] (innermost first), boxes of 64 columns
 // x 128 rows with 128-byte swizzle; rows past `slots` read as zeros.
@@ -1020,8 +1045,9 @@ int32_t prepare_device(int dev) {
   tc_cluster_capacity(dev);
   if (tensor_map_encoder() == nullptr) return SINK_EDEVICE;
   void* scratch = nullptr;  // the no-allocation entry point's static array, on this device
-  const int32_t rc = noalloc_scratch(dev, &scratch);
+  int32_t rc = noalloc_scratch(dev, &scratch);
   if (rc) return rc;
+  if ((rc = prepare_paged(dev))) return rc;
   g_prepared.fetch_or(bit, std::memory_order_acq_rel);
   return SINK_OK;
 }

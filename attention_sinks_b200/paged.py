@@ -1,0 +1,156 @@
+"""Paged K/V cache for a batch of sequences that may share a long prefix: append with the
+rotation applied on the way, and decode attention that reads the shared rows once.
+
+A sink cache gives every stream its own buffer of fixed length.  Here rows live in pages of a
+pool, a sequence's pages are named by its row of a block table, and several sequences may name
+the same pages: a prompt that a whole batch starts from is stored once, and
+`PagedKVCache.attend(..., shared_len=P)` computes the attention over its P rows for all
+queries together (one pass over those keys and values per kv head), merged with each
+sequence's own rows.
+
+One decode step of one layer:
+
+    lens += 1                                     # once per step, for all layers
+    q = cache.append(k, v, q=q)                   # rows lens - 1, rotated there; q rotated too
+    out = cache.attend(q, shared_len=prefix)      # [B, 1, Hq, D]
+
+Block table, lengths and counts are device tensors that the kernels read, so a captured CUDA
+graph of the step serves every later token.
+"""
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .rope import _rotation, device_frequencies
+
+# Scratch of `attend`, one buffer per (device, stream): calls on one stream run in order, so they
+# can share one.  Inside a graph capture a fresh one comes from the graph's own pool, so that
+# two graphs never share.
+_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, _lib.stream_handle(device))
+    buf = _SCRATCH.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = _SCRATCH[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf
+
+
+class PagedKVCache:
+    """One layer's paged cache over tensors of the caller's.
+
+    k_pages, v_pages: [pages, Hkv, page_size, D] pools (rows contiguous, page and head strides
+    free), bfloat16, float16 or float32.  block_table: int32 [B, width]; row p of sequence b is
+    slot p % page_size of page block_table[b, p // page_size].  lens: int32 [B], the rows of each
+    sequence, this step's tokens included; 0 for an idle sequence.  Both are read by the kernels
+    when they run: update them in place.  Layers of one model share them, and may share `status`
+    (a device int32 word that failures are recorded in).
+
+    inv_freq (or None: keys and queries are stored and returned as they are), interleaved and
+    attention_scaling are `rotary`'s.
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                 inv_freq: torch.Tensor | None = None, interleaved: bool = False, attention_scaling: float = 1.0,
+                 status: torch.Tensor | None = None):
+        device = k_pages.device
+        _lib.check_device(device)
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+            raise ValueError(f"pools are [pages, Hkv, page_size, D] of one shape and type, got {tuple(k_pages.shape)} "
+                             f"{k_pages.dtype}, {tuple(v_pages.shape)} {v_pages.dtype}")
+        pages, hkv, page, d = k_pages.shape
+        for x in (k_pages, v_pages):
+            if x.stride(-1) != 1 or (page > 1 and x.stride(-2) != d):
+                raise ValueError("pages need contiguous rows (stride[-2] == head_dim, stride[-1] == 1)")
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(-1) != 1:
+            raise ValueError("block_table is an int32 [B, width] tensor with a unit last stride")
+        batch, width = block_table.shape
+        if lens.shape != (batch,) or lens.dtype != torch.int32 or not lens.is_contiguous():
+            raise ValueError(f"lens is a contiguous int32 [{batch}] tensor")
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=device)
+        elif status.dtype != torch.int32 or status.numel() != 1:
+            raise ValueError("status is one int32 word")
+        for x in (v_pages, block_table, lens, status):
+            if x.device != device:
+                raise ValueError(f"the cache's tensors are on one device, got {device} and {x.device}")
+        if inv_freq is not None and 2 * inv_freq.numel() > d:
+            raise ValueError(f"{2 * inv_freq.numel()} rotated dims of a head of {d}")
+        self.k_pages, self.v_pages, self.block_table, self.lens, self.status = k_pages, v_pages, block_table, lens, status
+        self.device, self.dtype = device, k_pages.dtype
+        self.batch, self.heads_kv, self.page_size, self.head_dim = batch, hkv, page, d
+        self.inv_freq = None if inv_freq is None else device_frequencies(inv_freq, device)
+        self._rot = None if inv_freq is None else _rotation(self.inv_freq, interleaved, attention_scaling, False)
+        self._kv = _lib.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lens.data_ptr(),
+                                status.data_ptr(), _lib.dtype_code(k_pages.dtype), batch, hkv, d, page, pages, width, 0,
+                                block_table.stride(0), k_pages.stride(0), k_pages.stride(1), v_pages.stride(0),
+                                v_pages.stride(1))
+        _lib.prepare_device(device)  # before any graph capture of this cache's steps
+
+    def _rows(self, name: str, x: torch.Tensor, heads: int | None, tokens: int) -> torch.Tensor:
+        """x as the kernels take it, [B, heads, tokens, D] with a unit last stride."""
+        if (x.dim() != 4 or x.shape[0] != self.batch or (heads is not None and x.shape[1] != heads)
+                or x.shape[2] != tokens or x.shape[3] != self.head_dim or x.dtype != self.dtype
+                or x.device != self.device):
+            raise ValueError(f"{name} is [{self.batch}, {heads or 'Hq'}, {tokens}, {self.head_dim}] {self.dtype} on "
+                             f"{self.device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"the paged cache keeps no gradients: call it under torch.no_grad() or detach {name}")
+        return x if x.stride(-1) == 1 else x.contiguous()
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
+               counts: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Store the first counts[b] (all, when None) of the tokens k, v [B, Hkv, T, D] as the last
+        rows of sequence b: rows lens[b] - counts[b] .. lens[b] - 1, k rotated to those
+        positions.  Returns q [B, Hq, T, D] rotated to them too, in one launch (None without q).
+        Tokens from counts[b] on, and all of an idle sequence's (lens 0), are not stored; their
+        q rows come back as zeros.  counts: int32 [B] on the device."""
+        tokens = k.shape[2] if k.dim() == 4 else -1
+        k, v = self._rows("k", k, self.heads_kv, tokens), self._rows("v", v, self.heads_kv, tokens)
+        if counts is not None and (counts.shape != (self.batch,) or counts.dtype != torch.int32
+                                   or counts.device != self.device or not counts.is_contiguous()):
+            raise ValueError(f"counts is a contiguous int32 [{self.batch}] tensor on {self.device}")
+        q_out = None
+        if q is not None:
+            q = self._rows("q", q, None, tokens)
+            q_out = torch.empty_like(q)
+        if tokens and self.batch:
+            with torch.cuda.device(self.device):
+                _lib.paged_append(self._kv, k, v, counts, q, q_out, self._rot)
+        return q_out
+
+    def attend(self, q: torch.Tensor, scale: float | None = None, shared_len: int = 0) -> torch.Tensor:
+        """Attention of one query token per sequence, q [B, Hq, 1, D], over its rows
+        [0, lens[b]): [B, 1, Hq, D] in q's type, zeros for an idle sequence.  `scale` defaults
+        to D ** -0.5.
+
+        The first `shared_len` rows (a multiple of the page size) are the same for all
+        sequences: they are read through the first row of the block table, once per kv head
+        for the whole batch.  bfloat16 or float16, head_dim 64 or 128, pages of 16, 32, 64 or
+        128 rows, up to 8 query heads per kv head."""
+        q = self._rows("q", q, None, 1)
+        b, hq, _, d = q.shape
+        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+            q = q.contiguous()  # the kernel's tiled copies start rows on 16-byte boundaries
+        out = torch.empty(b, 1, hq, d, dtype=q.dtype, device=self.device)
+        if b == 0:
+            return out
+        need = _lib.paged_workspace_bytes(b, self.heads_kv, hq, d, shared_len, _lib.sm_count(self.device))
+        with torch.cuda.device(self.device):
+            _lib.paged_attention(q, self._kv, shared_len, d ** -0.5 if scale is None else scale, out,
+                                 _scratch(max(need, 256), self.device))
+        return out
+
+    def check_status(self) -> None:
+        """Raise RuntimeError if a kernel met a position past the block table or a page outside
+        the pool since the last check (nothing was accessed there); synchronises the stream."""
+        st = ctypes.c_int32(0)
+        with torch.cuda.device(self.device):
+            _lib._check(_lib.lib().sink_read_status(self.status.data_ptr(), _lib.stream_handle(self.device),
+                                                    ctypes.byref(st)), "sink_read_status")
+        _lib.raise_status(st.value)

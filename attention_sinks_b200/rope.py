@@ -6,13 +6,21 @@ Rotations compose by adding angles, so a key rotated at position p and then by -
 the key rotated at p - delta: that is what lets the sink cache move kept keys to new
 positions after an eviction (src/sinkcache/rope.py:1-14).
 
-These are the host-side helpers of the package: `rope_cos_sin` builds the fp32 cos/sin
-tables the eviction kernel consumes (one [head_dim] table per shift), exactly as
+The host-side helpers of the package: `rope_cos_sin` builds the fp32 cos/sin tables the
+eviction kernel consumes (one [head_dim] table per shift), exactly as
 src/sinkcache/rope.py:24-28 does; `apply_rope` / `rerotate` keep the reference's public
 helpers (src/sinkcache/rope.py:43-54) for users and tests.
+
+`rotary` is the rotation on the GPU: q and k in one kernel launch, half-split or interleaved
+pairs, a part of the head, fp64 angles, with its backward pass.  `rope_frequencies` gives the
+frequencies it takes, scaled for long contexts where asked.
 """
 
+import math
+
 import torch
+
+from . import _lib
 
 
 def rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -52,3 +60,144 @@ def rerotate(keys: torch.Tensor, delta: int, inv_freq: torch.Tensor) -> torch.Te
     (src/sinkcache/rope.py:49-54)."""
     cos, sin = rope_cos_sin(torch.tensor(-delta, device=keys.device), inv_freq.to(keys.device))
     return _rotate(keys, cos, sin)
+
+
+# ------------------------------------------------------------------ rotation on the GPU
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, kind: str = "default", factor: float = 1.0,
+                     original_length: int = 8192, length: int | None = None, low_freq_factor: float = 1.0,
+                     high_freq_factor: float = 4.0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0) -> tuple[torch.Tensor, float]:
+    """(float64 inverse frequencies [rot_dim / 2], attention scaling) of a rotary embedding.
+
+    base ** (-2i / rot_dim), then, for contexts `factor` times the `original_length` the model
+    was trained on:
+      "linear"   every frequency divided by factor (positions interpolated);
+      "ntk"      the base raised so that the lowest frequency reaches a context of `length` (the
+                 original length times factor when not given);
+      "llama3"   wavelengths above original_length / low_freq_factor divided by factor, those
+                 below original_length / high_freq_factor kept, a linear blend between;
+      "yarn"     pairs that turn more than beta_fast times over the original length kept, those
+                 that turn less than beta_slow times divided by factor, a ramp over the pair
+                 index between; attention scaling 0.1 ln(factor) + 1."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be a positive even number, got {rot_dim}")
+    if factor < 1.0:
+        raise ValueError(f"a context is extended by a factor of 1 or more, got {factor}")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    f = base ** (-i / rot_dim)
+    if kind == "default":
+        return f, 1.0
+    if kind == "linear":
+        return f / factor, 1.0
+    if kind == "ntk":
+        reach = max(length if length is not None else factor * original_length, original_length) / original_length
+        if rot_dim == 2:
+            return f, 1.0
+        raised = base * (factor * reach - (factor - 1.0)) ** (rot_dim / (rot_dim - 2))
+        return raised ** (-i / rot_dim), 1.0
+    if kind == "llama3":
+        turns = original_length * f / (2 * math.pi)
+        keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0.0, 1.0)
+        return f * keep + f / factor * (1.0 - keep), 1.0
+    if kind == "yarn":
+        def pair_turning(turns):  # the (fractional) pair that turns so often over the original length
+            return rot_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low = max(math.floor(pair_turning(beta_fast)), 0)
+        high = min(math.ceil(pair_turning(beta_slow)), rot_dim - 1)
+        ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        return f * (1.0 - ramp) + f / factor * ramp, (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+    raise ValueError(f"unknown kind of frequency scaling {kind!r}")
+
+
+def _rotation(inv_freq: torch.Tensor, interleaved: bool, scale: float, inverse: bool) -> "_lib.Rotation":
+    return _lib.Rotation(inv_freq.data_ptr(), inv_freq.numel(), int(interleaved), float(scale), int(inverse))
+
+
+def device_frequencies(inv_freq: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """`inv_freq` as the kernels read it: contiguous float64 on `device` (itself, if it is that)."""
+    if inv_freq.dim() != 1:
+        raise ValueError(f"inv_freq is one-dimensional, got {tuple(inv_freq.shape)}")
+    return inv_freq.detach().to(device, torch.float64).contiguous()
+
+
+def _launch(q, k, positions, inv_freq, interleaved, scale, inverse):
+    outs = []
+    ins = []
+    for x in (q, k):
+        if x is not None and x.stride(-1) != 1:
+            x = x.contiguous()
+        ins.append(x)
+        outs.append(torch.empty_like(x) if x is not None else None)
+    if q.numel() or (k is not None and k.numel()):
+        with torch.cuda.device(q.device):
+            _lib.rotary(ins[0], outs[0], ins[1], outs[1], positions,
+                        _rotation(inv_freq, interleaved, scale, inverse))
+    return outs[0], outs[1]
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation is linear and (up to the attention scaling) orthogonal, so its backward
+    pass is the rotation of the gradients by the negative angles: the same kernel, and itself
+    differentiable."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = interleaved, scale, inverse
+        q_out, k_out = _launch(q, k, positions, inv_freq, interleaved, scale, inverse)
+        return (q_out, k_out) if k is not None else q_out
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        positions, inv_freq = ctx.saved_tensors
+        interleaved, scale, inverse = ctx.how
+        rest = (positions, inv_freq, interleaved, scale, not inverse)
+        if dq is not None and dk is not None:
+            dq, dk = _Rotary.apply(dq, dk, *rest)
+        elif dq is not None:
+            dq = _Rotary.apply(dq, None, *rest)
+        elif dk is not None:
+            dk = _Rotary.apply(dk, None, *rest)
+        return dq, dk, None, None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+           interleaved: bool = False, attention_scaling: float = 1.0):
+    """Rotate q [B, Hq, T, D] and k [B, Hkv, T, D] (or None) at `positions` ([T] or [B, T]) by
+    the angles positions * inv_freq, in one kernel launch; returns (q_rot, k_rot), new tensors
+    in the layout of the inputs (k_rot None without k).  Differentiable in q and k.
+
+    The first 2 * len(inv_freq) dims are rotated, the rest copied.  Pairs are (i, i + half), or
+    (2i, 2i + 1) with `interleaved`.  Angles are formed in float64, the rotation in float32 with
+    one rounding to the tensors' type (float32, bfloat16 or float16); cos and sin are multiplied
+    by `attention_scaling`.  An inv_freq that is not float64 on the device is converted per call.
+    Forward and backward can be captured into a CUDA graph, on torch's terms: no autograd graph
+    of the same leaf tensors made outside the capture may be alive.
+    """
+    if q.dim() != 4:
+        raise ValueError(f"q is [B, H, T, D], got {tuple(q.shape)}")
+    device = q.device
+    _lib.check_device(device)
+    _lib.dtype_code(q.dtype)
+    b, _, t, d = q.shape
+    if k is not None and (k.dim() != 4 or k.shape[0] != b or k.shape[2] != t or k.shape[3] != d
+                          or k.dtype != q.dtype or k.device != device):
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} {k.device} does not go with q {tuple(q.shape)} {q.dtype} "
+                         f"{device}")
+    if positions.device != device or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"positions are whole numbers on {device}, got {positions.dtype} on {positions.device}")
+    if positions.shape not in ((t,), (b, t), (1, t)):
+        raise ValueError(f"positions are [{t}] or [{b}, {t}], got {tuple(positions.shape)}")
+    if 2 * inv_freq.numel() > d or d > 512:
+        raise ValueError(f"{2 * inv_freq.numel()} rotated dims of a head of {d} (at most 512)")
+    if positions.dtype != torch.int64 or (t > 1 and positions.stride(-1) != 1):
+        positions = positions.to(torch.int64).contiguous()
+    inv_freq = device_frequencies(inv_freq, device)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _Rotary.apply(q, k, positions, inv_freq, interleaved, attention_scaling, False)
+        return out if k is not None else (out, None)
+    return _launch(q, k, positions, inv_freq, interleaved, attention_scaling, False)

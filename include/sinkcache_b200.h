@@ -51,8 +51,9 @@ extern "C" {
 #define SINK_EDEVICE (-7)     /* no usable CUDA device */
 #define SINK_ESCRATCH (-8)    /* needs more than the static scratch of sink_decode_attention_noalloc */
 
-/* status bits written by kernels into the workspace status word */
+/* status bits written by kernels into the workspace (or paged cache) status word */
 #define SINK_STATUS_WAIT_TIMEOUT 1
+#define SINK_STATUS_BAD_PAGE 2 /* a position past the block table, or a page index out of range */
 
 /* operations, for sink_workspace_bytes() */
 #define SINK_OP_APPEND 0
@@ -363,6 +364,97 @@ int32_t sink_decode_attention_noalloc(const sink_rows_t* q, const sink_kv_buffer
                                       int32_t rows, float scale, const uint8_t* mask,
                                       int64_t mask_stride_b, void* out, int64_t out_stride_b,
                                       int64_t out_stride_h, void* stream);
+
+/*
+ * ---- Operators beside the sink caches: rotation, paged cache append, shared-prefix attention.
+ * No counterparts in the reference's kernels; sink_rotary does on the GPU, in one launch and
+ * with fp64 angles, what src/sinkcache/rope.py:24-54 does in elementary torch.
+ */
+
+/* A rotation of a head's first 2 * rot_half dims: angle of pair i at position p = p *
+ * inv_freq[i], formed in fp64; y1 = scale (x1 cos - x2 sin), y2 = scale (x2 cos + x1 sin). */
+typedef struct sink_rotation {
+  const double* inv_freq; /* device [rot_half] */
+  int32_t rot_half;       /* 0 .. 256, 2 * rot_half <= head_dim; the other dims pass through */
+  int32_t interleaved;    /* 0: pairs (x_i, x_{i + rot_half}); 1: pairs (x_{2i}, x_{2i+1}) */
+  float scale;            /* attention scaling on cos and sin (1 for none) */
+  int32_t inverse;        /* 1: rotate by the negative angles (the backward pass) */
+} sink_rotation_t;
+
+/*
+ * q_out = rotate(q), k_out = rotate(k) in one launch.  Each [batch, heads, n, head_dim] with a
+ * unit last stride and any other strides (0 included, for a source); q and k may differ in
+ * heads; k and k_out may both be NULL.  A destination may be its own source, element for
+ * element.  positions: device int64, of token t of sequence b at [b * positions_stride_b + t]
+ * (stride 0 shares one row).  head_dim <= 512; fp32, bf16 or fp16; fp32 arithmetic, one
+ * rounding to the type.
+ */
+int32_t sink_rotary(int32_t batch, int32_t head_dim, const sink_rows_t* q, const sink_rows_t* q_out,
+                    const sink_rows_t* k, const sink_rows_t* k_out, const int64_t* positions,
+                    int64_t positions_stride_b, const sink_rotation_t* rot, void* stream);
+
+/*
+ * One layer's paged K/V cache: pools of pages [pages, heads_kv, page_size, head_dim] whose rows
+ * are contiguous.  Row p of sequence b is slot p % page_size of page table[b][p / page_size].
+ * lens, table and status are device memory, read when the kernels run: a captured launch
+ * follows them.  A position past the table, or a page index outside [0, pages), is never
+ * accessed: it sets SINK_STATUS_BAD_PAGE in *status (an append skips the row; an attention's
+ * output for that sequence is void).
+ */
+typedef struct sink_paged_kv {
+  void* k;
+  void* v;
+  const int32_t* table; /* [batch][table_width], row stride table_stride */
+  const int32_t* lens;  /* [batch] rows of each sequence, this step's tokens included */
+  int32_t* status;      /* one word, zero at first */
+  int32_t dtype;
+  int32_t batch;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t pages;
+  int32_t table_width;
+  int32_t pad_;
+  int64_t table_stride;
+  int64_t k_stride_p; /* element strides between pages and between heads */
+  int64_t k_stride_h;
+  int64_t v_stride_p;
+  int64_t v_stride_h;
+} sink_paged_kv_t;
+
+/*
+ * Append: the first counts[b] tokens of k_new / v_new [batch, heads_kv, n, head_dim] become rows
+ * lens[b] - counts[b] .. lens[b] - 1 of sequence b, k rotated to its position on the way (rot
+ * NULL: as it is).  counts: device int32 [batch], NULL for n everywhere.  Tokens from counts[b]
+ * on, and tokens whose position is negative (an idle sequence: lens 0), are not written.
+ * q / q_out (both or neither; [batch, heads, n, head_dim]): rotated to the same positions in the
+ * same launch, zeros for tokens that are not written.  Two sequences that append to one slot
+ * leave one of the two rows there.
+ */
+int32_t sink_paged_append(const sink_paged_kv_t* kv, const sink_rows_t* k_new,
+                          const sink_rows_t* v_new, const int32_t* counts, const sink_rows_t* q,
+                          const sink_rows_t* q_out, const sink_rotation_t* rot, void* stream);
+
+/*
+ * Workspace of sink_paged_attention (0 for shapes it refuses).  It needs no initial value and
+ * keeps nothing between calls; calls that can overlap need one each.  Pure host arithmetic.
+ */
+size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads_q,
+                                  int32_t head_dim, int32_t shared_len, int32_t num_sms);
+
+/*
+ * Decode attention of one query token per sequence over its rows [0, lens[b]):
+ *   out[b, 0, hq, :] = softmax(q[b, hq] . K^T * scale) @ V,   zeros where lens[b] <= 0.
+ * The rows [0, shared_len) are the same for every sequence: they are read through
+ * table[0] (whatever the other rows of the table hold there), once per kv head for all
+ * queries; a sequence of fewer rows attends to its own number of them.  shared_len is a
+ * multiple of page_size, 0 for plain paged decode.  bf16 or fp16; head_dim 64 or 128;
+ * page_size 16, 32, 64 or 128; 1 to 8 query heads per kv head; page, head and q rows 16-byte
+ * aligned.
+ */
+int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, int32_t shared_len,
+                             float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

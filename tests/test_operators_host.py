@@ -1,0 +1,134 @@
+"""Argument checks of the rotation, paged-append and paged-attention entry points, made before
+anything is launched: no GPU needed."""
+
+import ctypes
+
+import pytest
+import torch
+
+from attention_sinks_b200 import PagedKVCache, _lib, rope_frequencies, rotary
+
+P = 4096  # a 16-byte aligned address that nothing reads
+
+
+def paged(**kw):
+    d = dict(k=P, v=P, table=P, lens=P, status=P, dtype=_lib.DTYPE_BF16, batch=2, heads_kv=2, head_dim=64, page_size=16,
+             pages=10, table_width=4, pad_=0, table_stride=4, k_stride_p=2048, k_stride_h=1024, v_stride_p=2048,
+             v_stride_h=1024)
+    d.update(kw)
+    return _lib.PagedKV(**d)
+
+
+def rows(heads=2, n=1, dtype=_lib.DTYPE_BF16, data=P, sb=None, sh=64, st=64):
+    return _lib.Rows(data, dtype, heads, n, 0, heads * 64 if sb is None else sb, sh, st)
+
+
+def attention(lib, kv, q=None, shared=0, out=P, sb=256, sh=64, ws=P, nbytes=1 << 30):
+    q = rows(heads=4) if q is None else q
+    return lib.sink_paged_attention(ctypes.byref(q), ctypes.byref(kv), shared, 0.125, out, sb, sh, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(k=None), _lib.EINVAL), (dict(table=None), _lib.EINVAL), (dict(lens=None), _lib.EINVAL),
+    (dict(status=None), _lib.EINVAL), (dict(batch=0), _lib.EINVAL), (dict(pages=0), _lib.EINVAL),
+    (dict(table_width=0), _lib.EINVAL), (dict(page_size=0), _lib.EINVAL), (dict(page_size=48), _lib.EINVAL),
+    (dict(page_size=128, table_width=1 << 26), _lib.EINVAL), (dict(dtype=_lib.DTYPE_F32), _lib.EDTYPE),
+    (dict(dtype=9), _lib.EDTYPE), (dict(dtype=_lib.DTYPE_F16), _lib.EDTYPE), (dict(head_dim=96), _lib.EHEADDIM),
+    (dict(head_dim=256), _lib.EHEADDIM), (dict(heads_kv=3), _lib.EGROUP), (dict(heads_kv=8), _lib.EGROUP),
+    (dict(k=P + 2), _lib.ELAYOUT), (dict(v_stride_p=2044), _lib.ELAYOUT), (dict(k_stride_h=-1024), _lib.ELAYOUT),
+])
+def test_paged_attention_refusals(built_lib, change, code):
+    assert attention(built_lib, paged(**change)) == code
+
+
+def test_paged_attention_refuses_queries_and_prefixes(built_lib):
+    lib = built_lib
+    assert attention(lib, paged(), q=rows(heads=4, n=2)) == _lib.EINVAL
+    assert attention(lib, paged(), q=rows(heads=18)) == _lib.EGROUP
+    assert attention(lib, paged(), q=rows(heads=4, data=P + 8)) == _lib.ELAYOUT
+    assert attention(lib, paged(), q=rows(heads=4, sh=65)) == _lib.ELAYOUT
+    for shared in (-16, 8, 80):  # negative, not whole pages, more than the table holds
+        assert attention(lib, paged(), shared=shared) == _lib.EINVAL
+    assert attention(lib, paged(), out=None) == _lib.EINVAL
+    assert attention(lib, paged(), ws=None) == _lib.EWORKSPACE
+    assert attention(lib, paged(), nbytes=16) == _lib.EWORKSPACE
+
+
+def test_workspace_is_host_arithmetic(built_lib):
+    need = _lib.paged_workspace_bytes
+    assert need(64, 8, 16, 128, 4096, 148) > 0
+    for bad in ((0, 8, 16, 128, 0, 148), (1, 8, 12, 128, 0, 148), (1, 1, 9, 128, 0, 148), (1, 8, 16, 96, 0, 148),
+                (1, 8, 16, 128, 0, 0), (1, 8, 16, 128, -128, 148), (1 << 23, 8, 16, 128, 0, 148)):
+        assert need(*bad) == 0
+
+
+def test_append_refusals(built_lib):
+    def call(kv, k=None, v=None, q=None, q_out=None, rot=None):
+        k, v = rows() if k is None else k, rows() if v is None else v
+        ref = lambda x: ctypes.byref(x) if x is not None else None  # noqa: E731
+        return built_lib.sink_paged_append(ctypes.byref(kv), ref(k), ref(v), None, ref(q), ref(q_out), ref(rot), None)
+
+    assert call(paged(lens=None)) == _lib.EINVAL
+    assert call(paged(), k=rows(heads=3)) == _lib.EINVAL
+    assert call(paged(), v=rows(n=2)) == _lib.EINVAL
+    assert call(paged(), k=rows(n=0), v=rows(n=0)) == _lib.EINVAL
+    assert call(paged(), k=rows(dtype=_lib.DTYPE_F16)) == _lib.EDTYPE
+    assert call(paged(), q=rows(heads=4)) == _lib.EINVAL  # nowhere to put it
+    assert call(paged(), q=rows(heads=4), q_out=rows(heads=2)) == _lib.EINVAL
+    assert call(paged(), rot=_lib.Rotation(P, 33, 0, 1.0, 0)) == _lib.EINVAL
+    assert call(paged(), rot=_lib.Rotation(None, 32, 0, 1.0, 0)) == _lib.EINVAL
+    assert call(paged(head_dim=1024), rot=None) == _lib.EHEADDIM
+    big = 1 << 30
+    assert call(paged(batch=4), k=rows(n=big), v=rows(n=big)) == _lib.EINVAL
+
+
+def test_rotary_refusals(built_lib):
+    def call(q=None, k=None, k_out=None, d=64, pos=P, rot=None, batch=1, q_out=None):
+        q = rows() if q is None else q
+        ref = lambda x: ctypes.byref(x) if x is not None else None  # noqa: E731
+        rot = _lib.Rotation(P, 32, 0, 1.0, 0) if rot is None else rot
+        return built_lib.sink_rotary(batch, d, ref(q), ref(q if q_out is None else q_out), ref(k), ref(k_out), pos, 0,
+                                     ref(rot), None)
+
+    assert call(batch=0) == _lib.EINVAL
+    assert call(pos=None) == _lib.EINVAL
+    assert call(k=rows()) == _lib.EINVAL
+    assert call(k=rows(n=3), k_out=rows(n=3)) == _lib.EINVAL
+    assert call(k=rows(dtype=_lib.DTYPE_F16), k_out=rows(dtype=_lib.DTYPE_F16)) == _lib.EDTYPE
+    assert call(q=rows(dtype=7)) == _lib.EDTYPE
+    assert call(q_out=rows(heads=1)) == _lib.EINVAL
+    assert call(d=600) == _lib.EHEADDIM
+    assert call(rot=_lib.Rotation(P, 64, 0, 1.0, 0)) == _lib.EINVAL
+    assert call(rot=_lib.Rotation(P, -1, 0, 1.0, 0)) == _lib.EINVAL
+    assert call(q=rows(n=1 << 30), batch=4) == _lib.EINVAL
+
+
+def test_host_tensors_are_refused():
+    f, _ = rope_frequencies(64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rotary(torch.zeros(1, 2, 3, 64), None, torch.arange(3), f)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        PagedKVCache(torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16, 64), torch.zeros(1, 2, dtype=torch.int32),
+                     torch.zeros(1, dtype=torch.int32))
+
+
+def test_rope_frequencies():
+    f, a = rope_frequencies(8, base=100.0)
+    assert a == 1.0 and f.dtype == torch.float64
+    torch.testing.assert_close(f, torch.tensor([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64))
+    torch.testing.assert_close(rope_frequencies(8, 100.0, "linear", 4.0)[0], f / 4)
+    ntk = rope_frequencies(64, kind="ntk", factor=1.0, original_length=4096, length=16384)[0]
+    plain = rope_frequencies(64)[0]
+    # the highest frequency stays, the lowest turns over 16,384 rows as it did over 4,096
+    assert ntk[0] == plain[0]
+    torch.testing.assert_close(ntk[-1] * 16384, plain[-1] * 4096)
+    l3 = rope_frequencies(64, 500000.0, "llama3", 32.0, 8192)[0]
+    base = rope_frequencies(64, 500000.0)[0]
+    assert torch.equal(l3[:8], base[:8]) and torch.equal(l3[-4:], base[-4:] / 32)
+    assert bool((l3[1:] < l3[:-1]).all())
+    yarn, a = rope_frequencies(64, kind="yarn", factor=16.0, original_length=4096)
+    assert abs(a - 1.2772588722239782) < 1e-12
+    assert yarn[0] == plain[0] and torch.equal(yarn[-1:], plain[-1:] / 16)
+    for bad in (dict(rot_dim=7), dict(rot_dim=0), dict(rot_dim=8, factor=0.5), dict(rot_dim=8, kind="other")):
+        with pytest.raises(ValueError):
+            rope_frequencies(**bad)
