@@ -84,13 +84,70 @@ int32_t dense_seg(RotSeg& s, const sink_rows_t* x, const sink_rows_t* y, int rot
   return SINK_OK;
 }
 
+// Elements per access: the largest power of two of at most 16 bytes that divides the pairs, the
+// head and every stride, and that every base address is aligned to.
+int rotate_vector(const RotArgs& A, int es) {
+  uint64_t bits = uint64_t(A.half) | uint64_t(A.D);
+  uint64_t addr = 0;
+  for (int i = 0; i < A.segs; ++i) {
+    const RotSeg& s = A.seg[i];
+    bits |= uint64_t(s.s_sb) | uint64_t(s.s_sh) | uint64_t(s.s_st) | uint64_t(s.d_sb) | uint64_t(s.d_sh) |
+            uint64_t(s.d_st);
+    addr |= reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst);
+  }
+  bits |= uint64_t(A.kp_s) | uint64_t(A.vp_s);
+  int vec = 16 / es;
+  while (vec > 1 && ((bits & uint64_t(vec - 1)) || (addr & uint64_t(vec * es - 1)))) vec >>= 1;
+  return vec;
+}
+
+constexpr int kRotRowsPerThread = 8;
+
+template <typename T, int VEC>
+int32_t launch_rotate_v(RotArgs A, int sms, cudaStream_t st) {
+  A.units = (A.half > 0 ? A.half : A.D) / VEC;
+  if (A.units > kRotThreads) A.units = kRotThreads;
+  const int slots = kRotThreads / A.units;
+  int heads = 0;
+  for (int i = 0; i < A.segs; ++i) heads += A.seg[i].heads;
+  // Rows per thread: what fills the device's CTA slots once, so that a small step is one wave
+  // with every load in flight, and at most kRotRowsPerThread, so that a large one has waves
+  // for the scheduler to even out.
+  const int64_t tokens = int64_t(A.batch) * A.tokens;
+  const int64_t threads = int64_t(sms) * kRotCtasPerSm * slots;
+  int64_t per = (tokens * heads + threads - 1) / threads;
+  per = per > kRotRowsPerThread ? kRotRowsPerThread : per;
+  int groups = int((heads + per - 1) / per);
+  if (groups > slots) groups = slots;
+  per = (heads + groups - 1) / groups;
+  A.groups = int((heads + per - 1) / per);  // the fewest teams of that many rows
+  A.team_tokens = slots / A.groups;
+  const dim3 grid(unsigned((tokens + A.team_tokens - 1) / A.team_tokens));
+  if (A.interleaved) return launch(sink_rotate_kernel<T, VEC, true>, grid, kRotThreads, 0, st, A);
+  return launch(sink_rotate_kernel<T, VEC, false>, grid, kRotThreads, 0, st, A);
+}
+
+template <typename T>
+int32_t launch_rotate_t(const RotArgs& A, int sms, cudaStream_t st) {
+  constexpr int kMax = 16 / int(sizeof(T));
+  const int vec = rotate_vector(A, int(sizeof(T)));
+  if (vec == kMax) return launch_rotate_v<T, kMax>(A, sms, st);
+  if (vec == kMax / 2) return launch_rotate_v<T, kMax / 2>(A, sms, st);
+  if constexpr (kMax == 8) {
+    if (vec == 2) return launch_rotate_v<T, 2>(A, sms, st);
+  }
+  return launch_rotate_v<T, 1>(A, sms, st);
+}
+
 int32_t launch_rotate(const RotArgs& A, int dtype, cudaStream_t st) {
   if (int64_t(A.batch) * A.tokens > INT_MAX) return SINK_EINVAL;
-  const dim3 grid(unsigned(A.batch * A.tokens));
+  int dev = 0;
+  const int sms = device_sms(&dev);
+  if (sms <= 0) return SINK_EDEVICE;
   switch (dtype) {
-    case SINK_DTYPE_BF16: return launch(sink_rotate_kernel<__nv_bfloat16>, grid, kRotThreads, 0, st, A);
-    case SINK_DTYPE_F16: return launch(sink_rotate_kernel<__half>, grid, kRotThreads, 0, st, A);
-    case SINK_DTYPE_F32: return launch(sink_rotate_kernel<float>, grid, kRotThreads, 0, st, A);
+    case SINK_DTYPE_BF16: return launch_rotate_t<__nv_bfloat16>(A, sms, st);
+    case SINK_DTYPE_F16: return launch_rotate_t<__half>(A, sms, st);
+    case SINK_DTYPE_F32: return launch_rotate_t<float>(A, sms, st);
     default: return SINK_EDTYPE;
   }
 }

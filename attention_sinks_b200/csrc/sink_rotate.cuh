@@ -19,6 +19,7 @@
 namespace sinkb200 {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotCtasPerSm = 4;  // CTAs of the kernel that an SM holds (64 registers a thread)
 constexpr int kRotMaxHalf = 256;  // pairs of a head at most (head_dim <= 512)
 
 // One tensor [batch, heads, tokens, D], its last dimension contiguous.
@@ -50,6 +51,9 @@ struct RotArgs {
   int table_width, page_size, pages;
   int64_t kp_s, vp_s;      // element strides between pages of k and v
   int* status;
+  // how the threads of a CTA share the work: `units` threads per row, `groups` teams of them
+  // per token (each takes every groups-th head), team_tokens tokens per CTA
+  int units, groups, team_tokens;
 };
 
 // cos and sin of p * f, |p * f| up to 2^52 or so: quarter turns are taken off in fp64, what is
@@ -66,28 +70,96 @@ __device__ __forceinline__ void rot_cos_sin(double p, double f, float& c, float&
   if (k >= 2) s = -s;
 }
 
-// One CTA per token: the angles' cos and sin once for all heads, then the heads' elements.
-template <typename T>
-__global__ void __launch_bounds__(kRotThreads) sink_rotate_kernel(const RotArgs A) {
+// N elements as one access of N * sizeof(T) bytes (a power of two, 16 at most).
+template <int BYTES>
+struct RotWord;
+template <>
+struct RotWord<16> { using type = uint4; };
+template <>
+struct RotWord<8> { using type = uint2; };
+template <>
+struct RotWord<4> { using type = uint32_t; };
+template <>
+struct RotWord<2> { using type = uint16_t; };
+
+template <typename T, int VEC>
+union RotVec {
+  typename RotWord<VEC * int(sizeof(T))>::type word;
+  T e[VEC];
+  __device__ __forceinline__ RotVec() {}
+};
+
+constexpr int kRotAhead = 2;  // rows whose loads a thread issues together
+
+// A thread owns VEC pairs of a token -- their cosines and sines stay in its registers -- and
+// walks rows (heads of all tensors, one after another): A.units threads cover a row's pairs,
+// A.groups such teams share a token's rows, and a CTA takes A.team_tokens tokens.  Per row and
+// thread two vectors of VEC elements are loaded and stored (16 bytes each where sizes and
+// alignment allow), the first rows' loads before the angles are formed.  The angles are formed
+// once per pair and team instead of once per pair and head, without barrier or shared memory.
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm) sink_rotate_kernel(const __grid_constant__ RotArgs A) {
   using E = Elem<T>;
-  __shared__ float2 cs[kRotMaxHalf];
+  using V = RotVec<T, VEC>;
+  using W = typename RotWord<VEC * int(sizeof(T))>::type;
   grid_dependency_wait();
   allow_dependents();
-  const int b = int(blockIdx.x) / A.tokens, t = int(blockIdx.x) - b * A.tokens;
+  const int slot_of = int(threadIdx.x) / A.units, unit = int(threadIdx.x) - slot_of * A.units;
+  const int token_of = slot_of / A.groups, group = slot_of - token_of * A.groups;
+  if (token_of >= A.team_tokens) return;
+  const unsigned token = blockIdx.x * unsigned(A.team_tokens) + token_of;  // batch * tokens < 2^31
+  if (token >= unsigned(A.batch) * unsigned(A.tokens)) return;
+  const int b = int(token / unsigned(A.tokens)), t = int(token - unsigned(b) * unsigned(A.tokens));
+  int count = A.tokens;
+  if (A.counts != nullptr) count = A.counts[b];
+  const int rows = A.seg[0].heads + A.seg[1].heads + A.seg[2].heads;  // unused segments have none
+
+  auto segment_of = [&](int r, int& h) {
+    int g = 0;
+    h = r;
+    if (h >= A.seg[0].heads) {
+      h -= A.seg[0].heads;
+      g = 1;
+      if (h >= A.seg[1].heads) {
+        h -= A.seg[1].heads;
+        g = 2;
+      }
+    }
+    return g;
+  };
+  // the pair's vectors: VEC elements half apart, or 2 * VEC consecutive ones
+  const int o1 = INTERLEAVED ? 2 * VEC * unit : VEC * unit;
+  const int o2 = INTERLEAVED ? o1 + VEC : o1 + A.half;
+  V x1[kRotAhead], x2[kRotAhead];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int j = 0; j < kRotAhead; ++j) {
+      const int r = r0 + j * A.groups;
+      if (r < rows) {
+        int h;
+        const RotSeg& S = A.seg[segment_of(r, h)];
+        const T* src = reinterpret_cast<const T*>(S.src) + b * S.s_sb + t * S.s_st + h * S.s_sh;
+        x1[j].word = *reinterpret_cast<const W*>(src + o1);
+        x2[j].word = *reinterpret_cast<const W*>(src + o2);
+      }
+    }
+  };
+  const bool in_count = t < count;
+  if (A.half > 0 && in_count) load(group);
+
   int64_t p;
   int64_t row_k = 0, row_v = 0;
   bool live = true;
   if (A.pos != nullptr) {
     p = A.pos[b * A.pos_sb + t];
   } else {
-    const int n = A.counts != nullptr ? A.counts[b] : A.tokens;
-    p = int64_t(A.lens[b]) - n + t;
-    live = t < n && p >= 0;
+    p = int64_t(A.lens[b]) - count + t;
+    live = in_count && p >= 0;
     if (live) {
       const int64_t at = p / A.page_size;
       const int page = at < A.table_width ? A.table[b * A.table_sb + at] : -1;
       if (page < 0 || page >= A.pages) {
-        if (threadIdx.x == 0) atomicOr(A.status, 2);
+        atomicOr(A.status, 2);
         live = false;
       } else {
         const int64_t slot = p - at * A.page_size;
@@ -96,32 +168,62 @@ __global__ void __launch_bounds__(kRotThreads) sink_rotate_kernel(const RotArgs 
       }
     }
   }
-  for (int i = threadIdx.x; i < A.half; i += kRotThreads) {
-    float c, s;
-    rot_cos_sin(static_cast<double>(p), A.inv_freq[i], c, s);
-    cs[i] = make_float2(c * A.scale, s * A.scale * A.sign);
-  }
-  __syncthreads();
-  for (int g = 0; g < A.segs; ++g) {
-    const RotSeg& S = A.seg[g];
-    if (!live && S.paged) continue;
-    const T* src = reinterpret_cast<const T*>(S.src) + b * S.s_sb + t * S.s_st;
-    T* dst = reinterpret_cast<T*>(S.dst) + (S.paged == 1 ? row_k : S.paged == 2 ? row_v : b * S.d_sb + t * S.d_st);
-    const int half = S.rotate ? A.half : 0;
-    const int per_row = A.D - half;  // a pair or a lone element each
-    for (int i = threadIdx.x; i < S.heads * per_row; i += kRotThreads) {
-      const int h = i / per_row, c = i - h * per_row;
-      const T* x = src + h * S.s_sh;
-      T* y = dst + h * S.d_sh;
-      if (c < half) {
-        const int i1 = A.interleaved ? 2 * c : c, i2 = A.interleaved ? 2 * c + 1 : c + half;
-        const float x1 = E::to_f(x[i1]), x2 = E::to_f(x[i2]);
-        const float2 w = cs[c];
-        y[i1] = E::from_f(live ? x1 * w.x - x2 * w.y : 0.f);
-        y[i2] = E::from_f(live ? x2 * w.x + x1 * w.y : 0.f);
-      } else {
-        y[c + half] = live ? x[c + half] : E::from_f(0.f);
+  auto dest = [&](const RotSeg& S, int h) {
+    return reinterpret_cast<T*>(S.dst) +
+           (S.paged == 1 ? row_k : S.paged == 2 ? row_v : b * S.d_sb + t * S.d_st) + h * S.d_sh;
+  };
+
+  if (A.half > 0) {
+    float c[VEC], s[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      rot_cos_sin(static_cast<double>(p), A.inv_freq[unit * VEC + i], c[i], s[i]);
+      c[i] *= A.scale;
+      s[i] *= A.scale * A.sign;
+    }
+    for (int r0 = group; r0 < rows; r0 += kRotAhead * A.groups) {
+      if (r0 != group && live) load(r0);
+#pragma unroll
+      for (int j = 0; j < kRotAhead; ++j) {
+        const int r = r0 + j * A.groups;
+        if (r >= rows) continue;
+        int h;
+        const RotSeg& S = A.seg[segment_of(r, h)];
+        if (!live && S.paged) continue;
+        T* dst = dest(S, h);
+        V y1, y2;
+        if (!live) {
+          y1.word = y2.word = W{};
+        } else if (S.rotate) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            // elements i of the two vectors, or pair i of their 2 * VEC consecutive ones
+            const int k1 = INTERLEAVED ? 2 * i : i, k2 = INTERLEAVED ? 2 * i + 1 : VEC + i;
+            const float a = E::to_f(k1 < VEC ? x1[j].e[k1 % VEC] : x2[j].e[k1 % VEC]);
+            const float d = E::to_f(k2 < VEC ? x1[j].e[k2 % VEC] : x2[j].e[k2 % VEC]);
+            (k1 < VEC ? y1 : y2).e[k1 % VEC] = E::from_f(a * c[i] - d * s[i]);
+            (k2 < VEC ? y1 : y2).e[k2 % VEC] = E::from_f(d * c[i] + a * s[i]);
+          }
+        } else {
+          y1.word = x1[j].word;
+          y2.word = x2[j].word;
+        }
+        *reinterpret_cast<W*>(dst + o1) = y1.word;
+        *reinterpret_cast<W*>(dst + o2) = y2.word;
       }
+    }
+  }
+  // the dims that pass through
+  if (2 * A.half < A.D) {
+    for (int r = group; r < rows; r += A.groups) {
+      int h;
+      const RotSeg& S = A.seg[segment_of(r, h)];
+      if (!live && S.paged) continue;
+      const T* src = reinterpret_cast<const T*>(S.src) + b * S.s_sb + t * S.s_st + h * S.s_sh;
+      T* dst = dest(S, h);
+#pragma unroll 4
+      for (int o = 2 * A.half + unit * VEC; o < A.D; o += A.units * VEC)
+        *reinterpret_cast<W*>(dst + o) = live ? *reinterpret_cast<const W*>(src + o) : W{};
     }
   }
 }

@@ -156,7 +156,11 @@ class _Rotary(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         interleaved, scale, inverse = ctx.how
         rest = (positions, inv_freq, interleaved, scale, not inverse)
-        if dq is not None and dk is not None:
+        if not torch.is_grad_enabled():  # no graph of the backward pass is asked for
+            if dq is None:
+                return None, (_launch(dk, None, *rest)[0] if dk is not None else None), None, None, None, None, None
+            dq, dk = _launch(dq, dk, *rest)
+        elif dq is not None and dk is not None:
             dq, dk = _Rotary.apply(dq, dk, *rest)
         elif dq is not None:
             dq = _Rotary.apply(dq, None, *rest)
