@@ -1,6 +1,8 @@
 // C ABI of the rotation, paged-append and paged-attention operators
 // (include/sinkcache_b200.h): argument checks and launches.
+#include <atomic>
 #include <climits>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/sinkcache_b200.h"
@@ -165,11 +167,94 @@ int32_t check_paged(const sink_paged_kv_t* c) {
   return SINK_OK;
 }
 
+// Workspace of one attention call.
+struct PagedPlan {
+  int per_tile = 0, tiles = 0;
+  size_t o_prefix = 0, ml_prefix = 0, o_own = 0, ml_own = 0, offsets = 0, total = 0;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+bool plan_paged(int64_t batch, int heads_kv, int heads_q, int D, int64_t shared, int sms, PagedPlan& p) {
+  if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || heads_q % heads_kv || heads_q / heads_kv > 8) return false;
+  if ((D != 64 && D != 128) || shared < 0 || sms < 1 || 4 * sms > kPgMaxParts) return false;
+  if (batch * heads_q > kPagedMaxRows) return false;
+  const int G = heads_q / heads_kv;
+  p.per_tile = int(batch < kPgTile / G ? batch : kPgTile / G);
+  p.tiles = int((batch + p.per_tile - 1) / p.per_tile);
+  // a piece of CTA c and unit u has slot c + u, with a partial for each of the two streams
+  const size_t slots_p = shared > 0 ? size_t(sms) + size_t(heads_kv) * ((p.tiles + 1) / 2) : 0;
+  const size_t slots_o = size_t(sms) + size_t(batch) * heads_kv;
+  size_t off = 0;
+  p.o_prefix = off;
+  off += align256(slots_p * 2 * kPgTile * D * 4);
+  p.ml_prefix = off;
+  off += align256(slots_p * 2 * kPgTile * 8);
+  p.o_own = off;
+  off += align256(slots_o * 2 * G * D * 4);
+  p.ml_own = off;
+  off += align256(slots_o * 2 * G * 8);
+  p.offsets = off;
+  off += align256((size_t(batch) + 2) * 4);
+  p.total = off;
+  return true;
+}
+
+int32_t encode(CUtensorMap* map, int32_t dtype, int rank, const void* data, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box) {
+  auto f = tensor_map_encoder();
+  if (f == nullptr) return SINK_EDEVICE;
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  const CUresult r = f(map, dtype == SINK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                       cuuint32_t(rank), const_cast<void*>(data), dims, strides, box, unit,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SINK_OK : SINK_ELAYOUT;
+}
+
+// A pool [pages, Hkv, page_size, D], boxes of 64 columns of one page.
+int32_t encode_pool(CUtensorMap* map, const void* data, const sink_paged_kv_t* c, int64_t stride_p, int64_t stride_h) {
+  const cuuint64_t row = cuuint64_t(c->head_dim) * 2;
+  const cuuint64_t sh = c->heads_kv > 1 ? cuuint64_t(stride_h) * 2 : row * c->page_size;
+  const cuuint64_t sp = c->pages > 1 ? cuuint64_t(stride_p) * 2 : sh * c->heads_kv;
+  const cuuint64_t dims[4] = {cuuint64_t(c->head_dim), cuuint64_t(c->page_size), cuuint64_t(c->heads_kv),
+                              cuuint64_t(c->pages)};
+  const cuuint64_t strides[3] = {row, sh, sp};
+  const cuuint32_t box[4] = {64, cuuint32_t(c->page_size), 1, 1};
+  return encode(map, c->dtype, 4, data, dims, strides, box);
+}
+
+// Queries [B, Hq, D], boxes of 64 columns x G heads x `seqs` sequences.
+int32_t encode_query(CUtensorMap* map, const sink_rows_t* q, int batch, int D, int G, int seqs) {
+  const cuuint64_t sh = q->heads > 1 ? cuuint64_t(q->stride_h) * 2 : cuuint64_t(D) * 2;
+  const cuuint64_t sb = batch > 1 ? cuuint64_t(q->stride_b) * 2 : sh * q->heads;
+  const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(q->heads), cuuint64_t(batch)};
+  const cuuint64_t strides[2] = {sh, sb};
+  const cuuint32_t box[3] = {64, cuuint32_t(G), cuuint32_t(seqs)};
+  return encode(map, q->dtype, 3, q->data, dims, strides, box);
+}
+
+template <typename T, int D>
+int32_t launch_paged_d(const PagedArgs& A, int heads_q, cudaStream_t st) {
+  const int32_t rc = launch(sink_paged_kernel<T, D>, dim3(unsigned(A.ctas)), kPgThreads, PgGeom<D>::kSmem, st, A);
+  if (rc) return rc;
+  return launch(sink_paged_combine_kernel<T, D>, dim3(unsigned(A.batch * heads_q)), D, 0, st, A);
+}
+
 template <typename T>
-int32_t launch_paged_t(int D, const PagedArgs& A, cudaStream_t st) {
-  const dim3 grid(unsigned(A.batch * A.heads_kv));
-  if (D == 64) return launch(sink_paged_simple_kernel<T, 64>, grid, 32 * A.group, 0, st, A);
-  return launch(sink_paged_simple_kernel<T, 128>, grid, 32 * A.group, 0, st, A);
+int32_t launch_paged_t(int D, const PagedArgs& A, int heads_q, cudaStream_t st) {
+  return D == 64 ? launch_paged_d<T, 64>(A, heads_q, st) : launch_paged_d<T, 128>(A, heads_q, st);
+}
+
+template <typename T>
+cudaError_t allow_paged_smem() {
+  cudaError_t e = cudaFuncSetAttribute(sink_paged_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       PgGeom<64>::kSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(sink_paged_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             PgGeom<128>::kSmem);
+  return e;
 }
 
 }  // namespace
@@ -177,7 +262,14 @@ int32_t launch_paged_t(int D, const PagedArgs& A, cudaStream_t st) {
 namespace sinkb200 {
 
 int32_t prepare_paged(int dev) {
-  (void)dev;
+  static std::atomic<uint64_t> done{0};  // one bit per device
+  const uint64_t bit = uint64_t(1) << dev;
+  if (done.load(std::memory_order_acquire) & bit) return SINK_OK;
+  cudaError_t e = allow_paged_smem<__nv_bfloat16>();
+  if (e == cudaSuccess) e = allow_paged_smem<__half>();
+  if (e != cudaSuccess) return e;
+  if (tensor_map_encoder() == nullptr) return SINK_EDEVICE;
+  done.fetch_or(bit, std::memory_order_acq_rel);
   return SINK_OK;
 }
 
@@ -278,49 +370,63 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   if (!aligned16(kv->k) || !aligned16(kv->v) || !aligned16(q->data)) return SINK_ELAYOUT;
   if ((kv->k_stride_p | kv->k_stride_h | kv->v_stride_p | kv->v_stride_h | q->stride_b | q->stride_h) & 7)
     return SINK_ELAYOUT;
+  const bool q_rows = (q->heads == 1 || q->stride_h >= D) && (kv->batch == 1 || q->stride_b >= D);
+  const bool k_rows = (kv->heads_kv == 1 || (kv->k_stride_h >= D && kv->v_stride_h >= D)) &&
+                      (kv->pages == 1 || (kv->k_stride_p >= D && kv->v_stride_p >= D));
+  if (!q_rows || !k_rows) return SINK_ELAYOUT;
+  if (!std::isfinite(scale)) return SINK_EINVAL;
+  // chunks of all sequences together stay in int
+  if (int64_t(kv->batch) * ((int64_t(kv->table_width) * page + kPgKeys - 1) / kPgKeys) > INT_MAX) return SINK_EINVAL;
   if (!workspace || workspace_bytes < 256 || !aligned16(workspace)) return SINK_EWORKSPACE;
   int dev = 0;
   const int sms = device_sms(&dev);
   if (sms <= 0) return SINK_EDEVICE;
-  if (workspace_bytes < sink_paged_workspace_bytes(kv->batch, kv->heads_kv, q->heads, D, shared_len, sms))
-    return SINK_EWORKSPACE;
+  PagedPlan plan;
+  if (!plan_paged(kv->batch, kv->heads_kv, q->heads, D, shared_len, sms, plan)) return SINK_EINVAL;
+  if (workspace_bytes < plan.total) return SINK_EWORKSPACE;
+  if ((rc = prepare_paged(dev))) return rc;
   PagedArgs A;
   std::memset(&A, 0, sizeof(A));
-  A.k = static_cast<const char*>(kv->k);
-  A.v = static_cast<const char*>(kv->v);
+  A.group = q->heads / kv->heads_kv;
+  if ((rc = encode_pool(&A.kmap, kv->k, kv, kv->k_stride_p, kv->k_stride_h))) return rc;
+  if ((rc = encode_pool(&A.vmap, kv->v, kv, kv->v_stride_p, kv->v_stride_h))) return rc;
+  if ((rc = encode_query(&A.qtile, q, kv->batch, D, A.group, plan.per_tile))) return rc;
+  if ((rc = encode_query(&A.qgroup, q, kv->batch, D, A.group, 1))) return rc;
   A.table = kv->table;
   A.lens = kv->lens;
   A.status = kv->status;
-  A.q = static_cast<const char*>(q->data);
   A.out = static_cast<char*>(out);
   A.table_sb = kv->table_stride;
-  A.k_sp = kv->k_stride_p;
-  A.k_sh = kv->k_stride_h;
-  A.v_sp = kv->v_stride_p;
-  A.v_sh = kv->v_stride_h;
-  A.q_sb = q->stride_b;
-  A.q_sh = q->stride_h;
   A.o_sb = out_stride_b;
   A.o_sh = out_stride_h;
+  char* ws = static_cast<char*>(workspace);
+  A.o_prefix = reinterpret_cast<float*>(ws + plan.o_prefix);
+  A.ml_prefix = reinterpret_cast<float2*>(ws + plan.ml_prefix);
+  A.o_own = reinterpret_cast<float*>(ws + plan.o_own);
+  A.ml_own = reinterpret_cast<float2*>(ws + plan.ml_own);
+  A.offsets = reinterpret_cast<int*>(ws + plan.offsets);
   A.batch = kv->batch;
   A.heads_kv = kv->heads_kv;
-  A.group = q->heads / kv->heads_kv;
   A.page_size = page;
   A.pages = kv->pages;
   A.table_width = kv->table_width;
   A.shared = shared_len;
-  A.scale_log2 = scale * kLog2e;
+  A.per_tile = plan.per_tile;
+  A.tiles = plan.tiles;
+  A.ctas = sms;
+  A.negate = scale < 0.f;
+  // a scale of 0 (uniform weights) becomes the smallest normal number, so that a masked score
+  // of -infinity stays one
+  A.scale_log2 = std::fmax(std::fabs(scale) * kLog2e, 1.17549435e-38f);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return kv->dtype == SINK_DTYPE_BF16 ? launch_paged_t<__nv_bfloat16>(D, A, st) : launch_paged_t<__half>(D, A, st);
+  return kv->dtype == SINK_DTYPE_BF16 ? launch_paged_t<__nv_bfloat16>(D, A, q->heads, st)
+                                      : launch_paged_t<__half>(D, A, q->heads, st);
 }
 
 size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads_q, int32_t head_dim,
                                   int32_t shared_len, int32_t num_sms) {
-  (void)shared_len;
-  if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || heads_q % heads_kv || heads_q / heads_kv > 8) return 0;
-  if ((head_dim != 64 && head_dim != 128) || num_sms < 1 || shared_len < 0) return 0;
-  if (int64_t(batch) * heads_q > kPagedMaxRows) return 0;
-  return 256;
+  PagedPlan plan;
+  return plan_paged(batch, heads_kv, heads_q, head_dim, shared_len, num_sms, plan) ? plan.total : 0;
 }
 
 }  // extern "C"

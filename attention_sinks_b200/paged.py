@@ -135,7 +135,7 @@ class PagedKVCache:
         128 rows, up to 8 query heads per kv head."""
         q = self._rows("q", q, None, 1)
         b, hq, _, d = q.shape
-        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8 or min(q.stride(0), q.stride(1)) < d:
             q = q.contiguous()  # the kernel's tiled copies start rows on 16-byte boundaries
         out = torch.empty(b, 1, hq, d, dtype=q.dtype, device=self.device)
         if b == 0:
