@@ -23,7 +23,8 @@
 // shared memory for 256 query rows; with one tile chunks alternate between the streams.  While
 // one warpgroup takes exponentials the tensor cores work for the other.  A thread owns a query
 // row (a TMEM lane): no reduction across threads.  P goes back to TMEM over its own scores,
-// 16-bit, and is the MMA's A operand from there.  The reference maximum only moves when a score
+// 16-bit, and is the MMA's A operand from there (one rounding to the cache's type: the tensor
+// cores take 16-bit operands; the sum of probabilities is of the unrounded ones).  The reference maximum only moves when a score
 // passes it by 2^8 (then O is rescaled in TMEM), so the usual chunk touches O in the MMA only.
 #pragma once
 
@@ -39,8 +40,10 @@ namespace sinkb200 {
 constexpr int kPgKeys = 128;      // keys per chunk
 constexpr int kPgTile = 128;      // query rows per tile
 constexpr int kPgThreads = 320;   // two softmax warpgroups, the MMA warp, the load warp
+constexpr int kPgNarrow = 8;      // query rows of a tile up to which four warps share its keys
 constexpr int kPgMmaWarp = 8, kPgLoadWarp = 9;
 constexpr float kPgRescale = 8.f; // log2
+constexpr int kPgP = 64;          // P's first column within its scores' 128
 constexpr int kPgTmemCols = 512;  // S of the streams at 0 and 128, O at 256 and 384
 
 template <int D>
@@ -48,7 +51,7 @@ struct PgGeom {
   static constexpr int kTileBytes = kPgKeys * D * 2;  // a K, V or Q tile: D / 64 boxes of 128 rows
   static constexpr int kBoxBytes = kPgKeys * 128;
   static constexpr int kRing = D == 128 ? 5 : 12;     // K and V tiles in flight
-  static constexpr int kBarBytes = 512;
+  static constexpr int kBarBytes = 1024;
   static constexpr int kSmem = 1024 + (2 + kRing) * kTileBytes + kBarBytes;
 };
 
@@ -240,6 +243,83 @@ __device__ __forceinline__ uint32_t pg_pack<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// exp2 arithmetic two elements at a time.
+__device__ __forceinline__ uint64_t pg_pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t pg_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t pg_add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float2 pg_two(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
+// 32 scores of a query row (fp32 bits), keys from `limit` on left out: -infinity.
+__device__ __forceinline__ void pg_mask(uint32_t (&r)[32], int limit) {
+  if (limit < 32) {
+#pragma unroll
+    for (int x = 0; x < 32; ++x)
+      if (x >= limit) r[x] = __float_as_uint(kNegInf);
+  }
+}
+
+__device__ __forceinline__ float pg_max(const uint32_t (&r)[32], float mx) {
+#pragma unroll
+  for (int x = 0; x < 32; ++x) mx = fmaxf(mx, __uint_as_float(r[x]));
+  return mx;
+}
+
+// Moves the row's reference maximum up to `mx` (log2 units) when that passes it by kPgRescale:
+// the sum and, if `has_o`, the row's O in TMEM are rescaled.  Rows that are no query (`valid`
+// false) compute along.
+template <int D>
+__device__ __forceinline__ void pg_reference(float mx, bool valid, bool has_o, uint32_t t_o, float& mref, float& l) {
+  const bool need = valid && mx > mref + kPgRescale;
+  if (!__any_sync(kFull, need)) return;
+  float alpha = 1.f;
+  if (need) {
+    alpha = pg_exp2(mref - mx);
+    mref = mx;
+    l *= alpha;
+  }
+  if (has_o) {  // (the last MMA on it is complete)
+#pragma unroll 1
+    for (int x = 0; x < D; x += 32) {
+      uint32_t o[32];
+      tc_ld32(t_o + x, o);
+      tc_wait_ld();
+#pragma unroll
+      for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+      tc_st32(t_o + x, o);
+    }
+  }
+}
+
+// Probabilities 2^(scale s - m) of 32 scores, their sum added to `sum` (two accumulators),
+// rounded to T and packed.
+template <typename T>
+__device__ __forceinline__ void pg_probs(const uint32_t (&r)[32], uint64_t scale2, uint64_t m2, uint64_t (&sum)[2],
+                                         uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const float2 e = pg_two(pg_fma2(pg_pair(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), scale2, m2));
+    const float p0 = pg_exp2(e.x), p1 = pg_exp2(e.y);
+    sum[x & 1] = pg_add2(sum[x & 1], pg_pair(p0, p1));
+    pk[x] = pg_pack<T>(p0, p1);
+  }
+}
+
 // ------------------------------------------------------------------ kernel
 
 template <typename T, int D>
@@ -252,14 +332,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   unsigned char* gbase = smem_raw + (base - raw);
   const uint32_t s_q = base, s_ring = base + 2 * kTB, s_bar = s_ring + kRing * kTB;
   const uint32_t b_full = s_bar, b_empty = b_full + 8 * kRing, b_qfull = b_empty + 8 * kRing, b_qempty = b_qfull + 16;
-  const uint32_t b_s = b_qempty + 16, b_p = b_s + 16, b_o = b_p + 16, b_done = b_o + 16;
+  const uint32_t b_s = b_qempty + 16, b_p = b_s + 16, b_o = b_p + 16, b_wg = b_o + 16, b_merge = b_wg + 16, b_done = b_merge + 32;
   unsigned char* g_bar = gbase + (s_bar - base);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(g_bar + 320);
-  int* flag = reinterpret_cast<int*>(g_bar + 324);
-  int* scan = reinterpret_cast<int*>(g_bar + 328);          // [10] warp sums
-  int* start = reinterpret_cast<int*>(g_bar + 368);         // first own sequence, chunks before it
-  int* any = reinterpret_cast<int*>(g_bar + 376);
-  static_assert(2 * 8 * kRing + 16 * 5 + 8 <= 320, "barriers");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(g_bar + 336);
+  int* flag = reinterpret_cast<int*>(g_bar + 340);
+  int* scan = reinterpret_cast<int*>(g_bar + 344);          // [12] warp sums
+  int* start = reinterpret_cast<int*>(g_bar + 392);         // first own sequence, chunks before it
+  int* any = reinterpret_cast<int*>(g_bar + 400);
+  float2* g_ml = reinterpret_cast<float2*>(g_bar + 512);    // [2 streams][4 warps][8 rows] of narrow tiles
+  static_assert(2 * 8 * kRing + 16 * 8 + 8 <= 336 && 512 + 2 * 4 * kPgNarrow * 8 <= G_::kBarBytes, "barriers");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -270,9 +351,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(b_qfull + 8 * i, 1);
       mbar_init(b_qempty + 8 * i, 1);
+      mbar_init(b_merge + 8 * i, 1);
+      mbar_init(b_merge + 16 + 8 * i, 1);
       mbar_init(b_s + 8 * i, 1);
       mbar_init(b_p + 8 * i, 128);
       mbar_init(b_o + 8 * i, 1);
+      mbar_init(b_wg + 8 * i, 128);
     }
     mbar_init(b_done, 1);
     *flag = 0;
@@ -374,11 +458,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   bool failed = false;
   PagedWalk walk = walk0;
   PagedPiece pc;
+  const bool narrow_prefix = A.tiles == 1 && A.batch * A.group <= kPgNarrow;
   if (warp == kPgLoadWarp) {
     // ================================================================ loads (the warp's lanes share a tile's pages)
     const int npg = kPgKeys / A.page_size;
     const int qrow_bytes = A.group * 128 * kBoxes;
-    int tile = 0, qseq = 0;  // ring tiles and Q tiles issued
+    int tile = 0, qseq = 0, step = 0;  // ring tiles, Q tiles and steps issued
+    // Per stream s and Q slot, at bit 2 s + slot: whether s merges in the slot's present tile
+    // (then the slot is free only after b_merge), and, 4 bits up, that barrier's parity.
+    uint32_t merges = 0;
     auto ring_slot = [&](int i) -> bool {  // waits until tile i's slot is free
       return i < kRing || pg_warp_wait(b_empty + 8 * (i % kRing), ((i / kRing) - 1) & 1);
     };
@@ -390,17 +478,30 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           failed = true;
           break;
         }
+        for (int x = slot; x < 4; x += 2) {
+          if (!((merges >> x) & 1u)) continue;
+          if (!pg_warp_wait(b_merge + 8 * x, (merges >> (4 + x)) & 1u)) failed = true;
+          merges ^= 0x11u << x;
+        }
+        if (failed) break;
+        if (pc.own || narrow_prefix) {
+          const int n = pc.j1 - pc.j0;
+          merges |= 1u << (2 * (step & 1) + slot);            // the stream of the first chunk
+          if (n > 1) merges |= 1u << (2 * (~step & 1) + slot);
+        }
         if (lane == 0) {
           const uint32_t bar = b_qfull + 8 * slot, dst = s_q + slot * kTB;
-          mbar_arrive_expect_tx(bar, pc.own ? qrow_bytes : qrow_bytes * A.per_tile);
-          for (int x = 0; x < kBoxes; ++x) {
-            if (pc.own)
-              tma_load_3d(dst + x * kBox, &A.qgroup, 64 * x, pc.h * A.group, pc.which, bar);
-            else
-              tma_load_3d(dst + x * kBox, &A.qtile, 64 * x, pc.h * A.group, (pc.which + s) * A.per_tile, bar);
-          }
+          // a narrow tile's rows once for each warp of the warpgroup, 32 TMEM lanes apart
+          const int copies = pc.own || narrow_prefix ? 4 : 1;
+          const CUtensorMap* map = pc.own ? &A.qgroup : &A.qtile;
+          const int seq = pc.own ? pc.which : (pc.which + s) * A.per_tile;
+          mbar_arrive_expect_tx(bar, (pc.own ? qrow_bytes : qrow_bytes * A.per_tile) * copies);
+          for (int x = 0; x < kBoxes; ++x)
+            for (int c = 0; c < copies; ++c)
+              tma_load_3d(dst + x * kBox + c * 32 * 128, map, 64 * x, pc.h * A.group, seq, bar);
         }
       }
+      step += (pc.j1 - pc.j0) * nq;
       // rows [row0, end) of the sequence (of the shared part) through one row of the table
       const int row0 = pc.own ? paged_own_row(A, pc.len) : 0;
       const int end = pc.own ? pc.len : A.shared;
@@ -500,7 +601,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         const bool first = c.pc.pair ? c.j == c.pc.j0 : c.j - c.pc.j0 < 2;
 #pragma unroll
         for (int kk = 0; kk < kPgKeys / 16; ++kk)
-          tc_mma_ta(tmem + 256 + s * 128, tmem + s * kPgKeys + kk * 8, tc_desc(vb + kk * 2048, kBox), idesc_o,
+          tc_mma_ta(tmem + 256 + s * 128, tmem + s * kPgKeys + kPgP + kk * 8, tc_desc(vb + kk * 2048, kBox), idesc_o,
                     !(first && kk == 0));
         if (!c.pc.pair || c.t == 1) tc_commit(b_empty + 8 * (i % kRing));
         if (c.pc.pair ? c.j + 1 == c.pc.j1 : c.j + 2 >= c.pc.j1) tc_commit(b_o + 8 * s);
@@ -526,10 +627,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     }
   } else {
     // ================================================================ softmax: warpgroup s, a thread per query row
-    const int s = warp >> 2, row = tid & 127;
-    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const int s = warp >> 2, row = tid & 127, wq = warp & 3;
+    const uint32_t lanes = uint32_t(wq * 32) << 16;
     const uint32_t t_s = tmem + s * kPgKeys + lanes, t_o = tmem + 256 + s * 128 + lanes;
-    int step = 0, chunk = 0, items = 0;  // steps and chunks before this piece; pieces this stream had steps of
+    int step = 0, chunk = 0, qseq = 0;  // steps, chunks and Q tiles before this piece
+    int items = 0, syncs = 0;           // pieces this stream had steps of; barriers of the warpgroup
+    auto wg_sync = [&]() -> bool {      // the warpgroup's threads, bounded
+      mbar_arrive(b_wg + 8 * s);
+      return pg_warp_wait(b_wg + 8 * s, (syncs++) & 1);
+    };
+    // whether prefix row r of tile `tile` belongs to a sequence that has the whole prefix
+    auto takes_part = [&](int tile, int r) { return paged_len(A, tile * A.per_tile + r / A.group) >= A.shared; };
     while (!failed && walk.next(A, L, pc)) {
       const int n = pc.j1 - pc.j0;
       const int t = (step & 1) ^ s;  // the tile, or the first of the piece's chunks, of this stream
@@ -541,7 +649,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         rows = A.group;
       else
         rows = imin(A.per_tile, A.batch - (pc.which + (pc.pair ? t : 0)) * A.per_tile) * A.group;
-      const bool idle = (warp & 3) * 32 >= rows;  // no row of this warp holds a query
+      const bool narrow = pc.own || narrow_prefix;  // warp wq of the warpgroup takes keys 32 wq .. 32 wq + 31
+      const bool idle = !narrow && wq * 32 >= rows;  // no row of this warp holds a query
       float mref = kNegInf, l = 0.f;
       for (int c = pc.pair ? 0 : t; c < n && !failed; c += inc) {
         const int st = pc.pair ? step + 2 * c + t : step + c;
@@ -567,56 +676,62 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           fence_proxy_async_smem();
         }
         tc_fence_after();
-        if (!idle) {
-          uint32_t r[kPgKeys];
-#pragma unroll
-          for (int x = 0; x < kPgKeys; x += 32) tc_ld32(t_s + x, r + x);
+        const uint64_t scale2 = pg_pair(A.scale_log2, A.scale_log2);
+        uint64_t sum[2] = {0, 0};
+        if (narrow) {
+          uint32_t r[32], pk[16], none[16];
+          tc_ld32(t_s + 32 * wq, r);
           tc_wait_ld();
-          if (limit < kPgKeys) {
+          pg_mask(r, limit - 32 * wq);
+          pg_reference<D>(pg_max(r, kNegInf) * A.scale_log2, lane < rows, c >= inc, t_o, mref, l);
+          const float m = mref == kNegInf ? 0.f : -mref;
+          pg_probs<T>(r, scale2, pg_pair(m, m), sum, pk);
 #pragma unroll
-            for (int x = 0; x < kPgKeys; ++x)
-              if (x >= limit) r[x] = __float_as_uint(kNegInf);
+          for (int x = 0; x < 16; ++x) none[x] = 0u;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // no probability for the other warps' keys
+            if (x == wq)
+              tc_st16(t_s + kPgP + 16 * x, pk);
+            else
+              tc_st16(t_s + kPgP + 16 * x, none);
           }
-          float mx = kNegInf;
-#pragma unroll
-          for (int x = 0; x < kPgKeys; ++x) mx = fmaxf(mx, __uint_as_float(r[x]));
-          mx *= A.scale_log2;
-          const bool need = row < rows && mx > mref + kPgRescale;
-          if (__any_sync(kFull, need)) {
-            float alpha = 1.f;
-            if (need) {
-              alpha = pg_exp2(mref - mx);
-              mref = mx;
-              l *= alpha;
-            }
-            if (c >= inc) {  // O holds this stream's earlier chunks (the last MMA on it is complete)
-#pragma unroll
-              for (int x = 0; x < D; x += 32) {
-                uint32_t o[32];
-                tc_ld32(t_o + x, o);
-                tc_wait_ld();
-#pragma unroll
-                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
-                tc_st32(t_o + x, o);
-              }
-            }
-          }
-          const float m = mref == kNegInf ? 0.f : mref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pk[kPgKeys / 2];
-#pragma unroll
-          for (int x = 0; x < kPgKeys; x += 2) {
-            const float p0 = pg_exp2(fmaf(__uint_as_float(r[x]), A.scale_log2, -m));
-            const float p1 = pg_exp2(fmaf(__uint_as_float(r[x + 1]), A.scale_log2, -m));
-            sum[x & 2] += p0;
-            sum[(x & 2) + 1] += p1;
-            pk[x / 2] = pg_pack<T>(p0, p1);  // rounded to the cache's type: the MMA's operand
-          }
-          tc_st32(t_s, pk);
-          tc_st32(t_s + 32, pk + 32);
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tc_wait_st();
+        } else if (!idle) {
+          // Once for the maximum, then again 32 at a time (the row's 128 scores would not fit
+          // the registers).  P takes the place of the last 64 scores, held in registers by then.
+          uint32_t x0[32], x1[32], pk[16];
+          tc_ld32(t_s, x0);
+          tc_ld32(t_s + 32, x1);
+          tc_wait_ld();
+          pg_mask(x0, limit);
+          pg_mask(x1, limit - 32);
+          float mx = pg_max(x1, pg_max(x0, kNegInf));
+          tc_ld32(t_s + 64, x0);
+          tc_ld32(t_s + 96, x1);
+          tc_wait_ld();
+          pg_mask(x0, limit - 64);
+          pg_mask(x1, limit - 96);
+          mx = pg_max(x1, pg_max(x0, mx));
+          pg_reference<D>(mx * A.scale_log2, row < rows, c >= inc, t_o, mref, l);
+          const float m = mref == kNegInf ? 0.f : -mref;
+          const uint64_t m2 = pg_pair(m, m);
+          pg_probs<T>(x0, scale2, m2, sum, pk);
+          tc_st16(t_s + kPgP + 32, pk);
+          tc_ld32(t_s, x0);
+          pg_probs<T>(x1, scale2, m2, sum, pk);
+          tc_st16(t_s + kPgP + 48, pk);
+          tc_wait_ld();
+          tc_ld32(t_s + 32, x1);
+          pg_mask(x0, limit);
+          pg_probs<T>(x0, scale2, m2, sum, pk);
+          tc_st16(t_s + kPgP, pk);
+          tc_wait_ld();
+          pg_mask(x1, limit - 32);
+          pg_probs<T>(x1, scale2, m2, sum, pk);
+          tc_st16(t_s + kPgP + 16, pk);
         }
+        const float2 add = pg_two(pg_add2(sum[0], sum[1]));
+        l += add.x + add.y;
+        tc_wait_st();
         tc_fence_before();
         mbar_arrive(b_p + 8 * s);
       }
@@ -625,25 +740,53 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         if (!pg_warp_wait(b_o + 8 * s, items & 1)) failed = true;
         ++items;
         tc_fence_after();
-        if (!idle && !failed) {
-          const size_t slot = size_t(int(blockIdx.x) + pc.unit) * 2 + t;
-          float* o_to;
-          float2* ml_to;
-          bool counts = row < rows;
-          if (pc.own) {
-            o_to = A.o_own + (slot * A.group + row) * D;
-            ml_to = A.ml_own + slot * A.group + row;
-          } else {
-            o_to = A.o_prefix + (slot * kPgTile + row) * D;
-            ml_to = A.ml_prefix + slot * kPgTile + row;
-            if (counts) {  // a sequence without the whole prefix does not take part
-              const int b = (pc.which + (pc.pair ? t : 0)) * A.per_tile + row / A.group;
-              if (paged_len(A, b) < A.shared) {
-                mref = kNegInf;
-                l = 0.f;
-              }
+        const size_t slot = size_t(int(blockIdx.x) + pc.unit) * 2 + t;
+        const int tile = pc.which + (pc.pair ? t : 0);
+        float* o_to = pc.own ? A.o_own + slot * A.group * D : A.o_prefix + slot * kPgTile * D;
+        float2* ml_to = pc.own ? A.ml_own + slot * A.group : A.ml_prefix + slot * kPgTile;
+        if (narrow) {
+          // The four warps' results over their keys, joined in shared memory: this stream's half
+          // of the piece's Q tile, which no MMA reads any more.
+          float* part = reinterpret_cast<float*>(gbase + (qseq & 1) * kTB + s * (kTB / 2));  // [4][8][D]
+          float2* ml = g_ml + s * 4 * kPgNarrow;
+          if (lane < rows) ml[wq * kPgNarrow + lane] = make_float2(mref, l);
+#pragma unroll
+          for (int x = 0; x < D; x += 32) {
+            uint32_t o[32];
+            tc_ld32(t_o + x, o);
+            tc_wait_ld();
+            if (lane < rows) {  // 16-byte words of a row turned by the row, against bank conflicts
+#pragma unroll
+              for (int y = 0; y < 32; y += 4)
+                *reinterpret_cast<uint4*>(part + (wq * kPgNarrow + lane) * D + (((x + y) >> 2) ^ lane) * 4) =
+                    make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
+          if (!wg_sync()) failed = true;
+          for (int i = row; i < rows * D; i += 128) {
+            const int g = i / D, d = i % D;
+            float m = kNegInf;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w * kPgNarrow + g].x);
+            float o = 0.f, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float2 v = ml[w * kPgNarrow + g];
+              if (v.x == kNegInf) continue;
+              const float f = pg_exp2(v.x - m);
+              o = fmaf(f, part[(w * kPgNarrow + g) * D + (((d >> 2) ^ g) << 2) + (d & 3)], o);
+              sum = fmaf(f, v.y, sum);
+            }
+            if (failed) break;
+            if (!pc.own && !takes_part(tile, g)) m = kNegInf;
+            o_to[i] = o;
+            if (d == 0) ml_to[g] = make_float2(m, sum);
+          }
+          fence_proxy_async_smem();  // the next Q tile there is written by TMA
+          if (!wg_sync()) failed = true;
+          if (row == 0) mbar_arrive(b_merge + 16 * s + 8 * (qseq & 1));  // done with its half of the Q tile
+        } else if (!idle && !failed) {
+          const bool counts = row < rows;
 #pragma unroll
           for (int x = 0; x < D; x += 32) {
             uint32_t o[32];
@@ -652,13 +795,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             if (counts) {
 #pragma unroll
               for (int y = 0; y < 32; y += 4)
-                *reinterpret_cast<uint4*>(o_to + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                *reinterpret_cast<uint4*>(o_to + row * D + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
-          if (counts) *ml_to = make_float2(mref, l);
+          // a sequence without the whole prefix does not take part
+          if (counts) ml_to[row] = takes_part(tile, row) ? make_float2(mref, l) : make_float2(kNegInf, 0.f);
         }
         tc_fence_before();
       }
+      qseq += pc.pair ? 2 : 1;
       step += pc.pair ? 2 * n : n;
       chunk += n;
     }
