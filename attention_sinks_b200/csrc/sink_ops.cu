@@ -170,20 +170,26 @@ int32_t check_paged(const sink_paged_kv_t* c) {
 // Workspace of one attention call.
 struct PagedPlan {
   int per_tile = 0, tiles = 0;
-  size_t o_prefix = 0, ml_prefix = 0, o_own = 0, ml_own = 0, offsets = 0, total = 0;
+  int units = 0;  // of the prefix
+  size_t o_prefix = 0, ml_prefix = 0, o_own = 0, ml_own = 0, bounds = 0, total = 0;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// Weights of a combine CTA: a float per query row and partial (two streams of the prefix pieces
+// and of the own pieces, at most one of each per CTA of the attention).
+size_t combine_smem(int sms, int G) { return size_t(4) * sms * G * 4; }
+
 bool plan_paged(int64_t batch, int heads_kv, int heads_q, int D, int64_t shared, int sms, PagedPlan& p) {
   if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || heads_q % heads_kv || heads_q / heads_kv > 8) return false;
-  if ((D != 64 && D != 128) || shared < 0 || sms < 1 || 4 * sms > kPgMaxParts) return false;
+  if ((D != 64 && D != 128) || shared < 0 || sms < 1 || combine_smem(sms, 8) > 48 * 1024) return false;
   if (batch * heads_q > kPagedMaxRows) return false;
   const int G = heads_q / heads_kv;
   p.per_tile = int(batch < kPgTile / G ? batch : kPgTile / G);
   p.tiles = int((batch + p.per_tile - 1) / p.per_tile);
   // a piece of CTA c and unit u has slot c + u, with a partial for each of the two streams
-  const size_t slots_p = shared > 0 ? size_t(sms) + size_t(heads_kv) * ((p.tiles + 1) / 2) : 0;
+  p.units = shared > 0 ? heads_kv * ((p.tiles + 1) / 2) : 0;
+  const size_t slots_p = shared > 0 ? size_t(sms) + p.units : 0;
   const size_t slots_o = size_t(sms) + size_t(batch) * heads_kv;
   size_t off = 0;
   p.o_prefix = off;
@@ -194,8 +200,8 @@ bool plan_paged(int64_t batch, int heads_kv, int heads_q, int D, int64_t shared,
   off += align256(slots_o * 2 * G * D * 4);
   p.ml_own = off;
   off += align256(slots_o * 2 * G * 8);
-  p.offsets = off;
-  off += align256((size_t(batch) + 2) * 4);
+  p.bounds = off;
+  off += align256((size_t(p.units) + size_t(batch) * heads_kv) * 8);
   p.total = off;
   return true;
 }
@@ -236,15 +242,16 @@ int32_t encode_query(CUtensorMap* map, const sink_rows_t* q, int batch, int D, i
 }
 
 template <typename T, int D>
-int32_t launch_paged_d(const PagedArgs& A, int heads_q, cudaStream_t st) {
+int32_t launch_paged_d(const PagedArgs& A, cudaStream_t st) {
   const int32_t rc = launch(sink_paged_kernel<T, D>, dim3(unsigned(A.ctas)), kPgThreads, PgGeom<D>::kSmem, st, A);
   if (rc) return rc;
-  return launch(sink_paged_combine_kernel<T, D>, dim3(unsigned(A.batch * heads_q)), D, 0, st, A);
+  return launch(sink_paged_combine_kernel<T, D>, dim3(unsigned(A.batch * A.heads_kv)), kPgCombineThreads,
+                int(combine_smem(A.ctas, A.group)), st, A);
 }
 
 template <typename T>
-int32_t launch_paged_t(int D, const PagedArgs& A, int heads_q, cudaStream_t st) {
-  return D == 64 ? launch_paged_d<T, 64>(A, heads_q, st) : launch_paged_d<T, 128>(A, heads_q, st);
+int32_t launch_paged_t(int D, const PagedArgs& A, cudaStream_t st) {
+  return D == 64 ? launch_paged_d<T, 64>(A, st) : launch_paged_d<T, 128>(A, st);
 }
 
 template <typename T>
@@ -404,7 +411,8 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   A.ml_prefix = reinterpret_cast<float2*>(ws + plan.ml_prefix);
   A.o_own = reinterpret_cast<float*>(ws + plan.o_own);
   A.ml_own = reinterpret_cast<float2*>(ws + plan.ml_own);
-  A.offsets = reinterpret_cast<int*>(ws + plan.offsets);
+  A.bounds = reinterpret_cast<int2*>(ws + plan.bounds);
+  A.units = plan.units;
   A.batch = kv->batch;
   A.heads_kv = kv->heads_kv;
   A.page_size = page;
@@ -419,8 +427,8 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   // of -infinity stays one
   A.scale_log2 = std::fmax(std::fabs(scale) * kLog2e, 1.17549435e-38f);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return kv->dtype == SINK_DTYPE_BF16 ? launch_paged_t<__nv_bfloat16>(D, A, q->heads, st)
-                                      : launch_paged_t<__half>(D, A, q->heads, st);
+  return kv->dtype == SINK_DTYPE_BF16 ? launch_paged_t<__nv_bfloat16>(D, A, st)
+                                      : launch_paged_t<__half>(D, A, st);
 }
 
 size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads_q, int32_t head_dim,
