@@ -48,25 +48,26 @@ namespace sinkb200 {
 constexpr int kPgKeys = 128;      // keys per chunk
 constexpr int kPgHalf = 64;       // keys per half step
 constexpr int kPgTile = 128;      // query rows per tile
-constexpr int kPgThreads = 320;   // two softmax warpgroups, the MMA warp, the load warp
-constexpr int kPgMmaWarp = 8, kPgLoadWarp = 9;
+constexpr int kPgThreads = 352;   // two softmax warpgroups, the load warp, two MMA warps
+constexpr int kPgLoadWarp = 8, kPgQkWarp = 9, kPgPvWarp = 10;
 constexpr int kPgNarrow = 8;      // query rows of a tile up to which four warps share its keys
 constexpr float kPgRescale = 8.f; // log2
 constexpr int kPgO = 256;         // TMEM: S of stream s, half h at 128 s + 64 h; O at 256 + 128 s
 constexpr int kPgTmemCols = 512;
-constexpr int kPgSteps = 16;      // step records in flight between the load and MMA warps
+constexpr int kPgSteps = 16;      // step records in flight between the load warp and the MMA warps
 
-// Shared memory: two wide Q tiles (or eight narrow ones, their 8-row blocks interleaved) | the
-// narrow tiles' merge area, half per stream | the ring of K and V tiles | barriers and records.
+// Shared memory: two wide Q tiles, or in the place of the first four narrow ones, their 8-row
+// blocks interleaved, and in that of the second the narrow tiles' merge area, half per stream |
+// the ring of K and V tiles | barriers and records.
 template <int D>
 struct PgGeom {
   static constexpr int kTileBytes = kPgKeys * D * 2;  // a K, V or Q tile: D / 64 boxes of 128 rows
   static constexpr int kBoxBytes = kPgKeys * 128;
   static constexpr int kMergeBytes = 2 * 4 * kPgNarrow * D * 4;
-  static constexpr int kRing = D == 128 ? 4 : 11;
+  static constexpr int kRing = D == 128 ? 5 : 12;     // K and V tiles in flight
   static constexpr int kBarBytes = 1152;
-  static constexpr int kSmem = 1024 + (2 + kRing) * kTileBytes + kMergeBytes + kBarBytes;
-  static_assert(kSmem <= 232448, "227 KB of shared memory");
+  static constexpr int kSmem = 1024 + (2 + kRing) * kTileBytes + kBarBytes;
+  static_assert(kMergeBytes <= kTileBytes && kSmem <= 232448, "227 KB of shared memory");
 };
 
 struct PagedArgs {
@@ -296,8 +297,8 @@ __device__ __forceinline__ float pg_max(const uint32_t (&r)[N], float mx) {
 }
 
 // Moves the row's reference maximum up to `mx` (log2 units) when that passes it by kPgRescale:
-// the sum and, if `has_o`, the row's O in TMEM are rescaled, once the last MMA on it (phase
-// parity `parity` of b_pv) is complete.  Rows that are no query (`valid` false) compute along.
+// the sum and, if `has_o`, the row's O in TMEM are rescaled, once the last MMA on it is
+// complete (phase parity `parity` of b_pv).  Rows that are no query (`valid` false) compute along.
 // False when a wait ran out.
 template <int D>
 __device__ __forceinline__ bool pg_reference(float mx, bool valid, bool has_o, uint32_t t_o, uint32_t b_pv,
@@ -340,14 +341,15 @@ __device__ __forceinline__ void pg_probs(const uint32_t (&r)[N], uint64_t scale2
   }
 }
 
-// What the MMA warp has to know of a step, written by the load warp.
+// What the MMA warps have to know of a step, written by the load warp.
 struct PgStep {
   static constexpr uint32_t kFirst = 1u, kLast = 2u;     // of the piece's steps on its stream
   static constexpr uint32_t kRelease = 4u;               // the last step on its chunk
   static constexpr uint32_t kQWait = 8u, kQRelease = 16u;// first, last use of the Q tile
   static constexpr uint32_t kMore = 32u;                 // another step on the same chunk follows
   static constexpr uint32_t kStop = 64u;                 // no step: the end
-  // bits 8..11: Q slot (0, 1 wide; 2.. narrow), bit 12: the slot's phase parity
+  // bits 8..11: Q slot (0, 1 wide; 2.. narrow), bit 12: the slot's phase parity, bits 16..: the
+  // tile's shared-memory address in 16-byte words
 };
 
 // ------------------------------------------------------------------ kernel
@@ -360,19 +362,19 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;  // swizzled tiles want 1024-byte alignment
   unsigned char* gbase = smem_raw + (base - raw);
-  const uint32_t s_q = base, s_merge = base + 2 * kTB, s_ring = s_merge + G_::kMergeBytes, s_bar = s_ring + kRing * kTB;
-  // mbarriers: full, empty [kRing]; qfull, qempty [10]; s, p, pv [stream * 2 + half]; wg [stream]; done
-  const uint32_t b_full = s_bar, b_empty = b_full + 8 * kRing, b_qfull = b_empty + 8 * kRing, b_qempty = b_qfull + 80;
-  const uint32_t b_s = b_qempty + 80, b_p = b_s + 32, b_pv = b_p + 32, b_wg = b_pv + 32, b_done = b_wg + 16;
+  const uint32_t s_q = base, s_ring = base + 2 * kTB, s_bar = s_ring + kRing * kTB;
+  // mbarriers: full, empty [kRing]; qfull, qempty [6]; s, p, pv [stream * 2 + half]; rec [4]; wg [stream]; done
+  const uint32_t b_full = s_bar, b_empty = b_full + 8 * kRing, b_qfull = b_empty + 8 * kRing, b_qempty = b_qfull + 48;
+  const uint32_t b_s = b_qempty + 48, b_p = b_s + 32, b_pv = b_p + 32, b_rec = b_pv + 32, b_wg = b_rec + 32, b_done = b_wg + 16;
   unsigned char* g_bar = gbase + (s_bar - base);
-  static_assert(16 * kRing + 160 + 96 + 16 + 8 <= 464, "barriers");
+  static_assert(16 * kRing + 96 + 128 + 16 + 8 <= 464, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(g_bar + 464);
   int* flag = reinterpret_cast<int*>(g_bar + 468);
   int* start = reinterpret_cast<int*>(g_bar + 472);               // first own sequence, chunks before it
-  int* scan = reinterpret_cast<int*>(g_bar + 480);                // [10] warp sums
-  float2* g_ml = reinterpret_cast<float2*>(g_bar + 520);          // [2 streams][4 warps][8 rows] of narrow tiles
-  uint32_t* steps = reinterpret_cast<uint32_t*>(g_bar + 520 + 2 * 4 * kPgNarrow * 8);  // [kPgSteps]
-  static_assert(520 + 2 * 4 * kPgNarrow * 8 + 4 * kPgSteps <= G_::kBarBytes, "records");
+  int* scan = reinterpret_cast<int*>(g_bar + 480);                // [11] warp sums
+  float2* g_ml = reinterpret_cast<float2*>(g_bar + 528);          // [2 streams][4 warps][8 rows] of narrow tiles
+  uint32_t* steps = reinterpret_cast<uint32_t*>(g_bar + 528 + 2 * 4 * kPgNarrow * 8);  // [kPgSteps]
+  static_assert(528 + 2 * 4 * kPgNarrow * 8 + 4 * kPgSteps <= G_::kBarBytes, "records");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 1);
     }
-    for (int i = 0; i < 10; ++i) {
+    for (int i = 0; i < 6; ++i) {
       mbar_init(b_qfull + 8 * i, 1);
       mbar_init(b_qempty + 8 * i, 1);
     }
@@ -388,9 +390,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       mbar_init(b_s + 8 * i, 1);
       mbar_init(b_p + 8 * i, 128);
       mbar_init(b_pv + 8 * i, 1);
+      mbar_init(b_rec + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(b_wg + 8 * i, 128);
-    mbar_init(b_done, 1);
+    mbar_init(b_done, 2);
     *flag = 0;
     start[0] = A.batch;
     start[1] = 0;
@@ -530,14 +533,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       const int nq = pc.pair ? 2 : 1;
       uint32_t q_bits[2] = {0, 0};
       for (int t = 0; t < nq && !failed; ++t) {
-        const int slot = narrow ? 2 + (thin & 7) : wide & 1, use = narrow ? thin >> 3 : wide >> 1;
+        const int slot = narrow ? 2 + (thin & 3) : wide & 1, use = narrow ? thin >> 2 : wide >> 1;
         if (use > 0 && !pg_warp_wait(b_qempty + 8 * slot, (use - 1) & 1)) {
           failed = true;
           break;
         }
         if (lane == 0) {
           const uint32_t bar = b_qfull + 8 * slot;
-          const uint32_t dst = narrow ? s_q + ((slot - 2) >> 2) * kTB + ((slot - 2) & 3) * 1024 : s_q + slot * kTB;
+          const uint32_t dst = s_q + (narrow ? (slot - 2) * 1024 : slot * kTB);
           // a narrow tile's rows once for each warp of the warpgroup, 32 TMEM lanes apart
           const int copies = narrow ? 4 : 1;
           const CUtensorMap* map = pc.own ? &A.qgroup : &A.qtile;
@@ -547,7 +550,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             for (int c = 0; c < copies; ++c)
               tma_load_3d(dst + x * kBox + c * 32 * 128, map, 64 * x, pc.h * A.group, seq, bar);
         }
-        q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12;
+        q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | ((s_q + (narrow ? (slot - 2) * 1024 : slot * kTB)) >> 4) << 16;
         narrow ? ++thin : ++wide;
       }
       for (int j = pc.j0; j < pc.j1 && !failed; ++j) {
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         page = next_page;
       }
     }
-    if (!failed) {  // tell the MMA warp that the steps end here
+    if (!failed) {  // tell the MMA warps that the steps end here
       if (!ring_slot(tile)) {
         failed = true;
       } else if (lane == 0) {
@@ -600,80 +603,102 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       for (int i = tile - 1; i >= 0 && i >= tile - kRing; --i)
         pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1);
       for (int i = wide - 1; i >= 0 && i >= wide - 2; --i) pg_warp_wait(b_qfull + 8 * (i & 1), (i >> 1) & 1);
-      for (int i = thin - 1; i >= 0 && i >= thin - 8; --i) pg_warp_wait(b_qfull + 8 * (2 + (i & 7)), (i >> 3) & 1);
+      for (int i = thin - 1; i >= 0 && i >= thin - 4; --i) pg_warp_wait(b_qfull + 8 * (2 + (i & 3)), (i >> 2) & 1);
     }
-  } else if (warp == kPgMmaWarp) {
-    // ================================================================ MMA issue (one lane)
+  } else if (warp == kPgQkWarp) {
+    // ================================================================ S = Q K^T (one lane)
     if (lane == 0) {
       constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc_s = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
-      constexpr uint32_t idesc_o = pg_idesc(kFmt, D, true);
-      const uint64_t kdesc = tc_desc(0, 16), vdesc = tc_desc(0, kBox);
-      // Half step m: half m & 1 of step m >> 1.  Scores run four half steps (two steps, one on
-      // each stream) ahead of the P V products: half step m's buffer is m - 4's.
-      int chunk = -1;            // of the newest step whose scores were issued
-      int pv_chunk = 0;
-      int last = INT_MAX;        // number of steps, once known
-      uint32_t rec = 0;          // record of that step
-      auto qk = [&](int m) -> bool {
-        const int n = m >> 1, h = m & 1, s = n & 1;
-        if (n >= last) return true;
-        if (h == 0) {
-          if (!(rec & PgStep::kMore)) {
-            ++chunk;
-            const int i = 2 * chunk;
-            if (!mbar_wait_bounded(b_full + 8 * (i % kRing), (i / kRing) & 1)) return false;
+      const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
+      const uint64_t desc = tc_desc(0, 16);
+      uint32_t rec = 0;
+      int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest step's K
+      for (int n = 0;; ++n) {
+        const int s = n & 1;
+        if (!(rec & PgStep::kMore)) {  // a chunk of its own
+          if ((r += 2) >= kRing) {
+            r -= kRing;
+            phase ^= 1;
           }
-          rec = steps[n % kPgSteps];
-          if (rec & PgStep::kStop) {
-            last = n;
-            return true;
+          if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
+            failed = true;
+            break;
           }
-          const uint32_t slot = (rec >> 8) & 15u;
-          if ((rec & PgStep::kQWait) && !mbar_wait_bounded(b_qfull + 8 * slot, (rec >> 12) & 1u)) return false;
         }
-        tc_fence_after();
-        const int i = 2 * chunk;
-        const uint32_t slot = (rec >> 8) & 15u;
-        const uint32_t q = slot < 2 ? s_q + slot * kTB : s_q + ((slot - 2) >> 2) * kTB + ((slot - 2) & 3) * 1024;
-        const uint64_t qd = kdesc + (q >> 4);
-        const uint64_t kd = kdesc + ((s_ring + (i % kRing) * kTB + h * kPgHalf * 128) >> 4);
-        const uint32_t d = tmem + s * 128 + h * kPgHalf;
+        rec = steps[n % kPgSteps];
+        mbar_arrive(b_rec + 8 * (n & 3));  // the P V warp may read it too
+        if (rec & PgStep::kStop) break;
+        if ((rec & PgStep::kQWait) && !mbar_wait_bounded(b_qfull + 8 * ((rec >> 8) & 15u), (rec >> 12) & 1u)) {
+          failed = true;
+          break;
+        }
+        const uint64_t qd = desc + (rec >> 16);
+        const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          constexpr int kStep = 32 >> 4;
-          const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * kStep;
-          tc_mma(d, qd + off, kd + off, idesc_s, kk > 0);
-        }
-        tc_commit(b_s + 8 * (2 * s + h));
-        if (h == 1) {
-          if (rec & PgStep::kRelease) tc_commit(b_empty + 8 * (i % kRing));
-          if (rec & PgStep::kQRelease) tc_commit(b_qempty + 8 * slot);
-        }
-        return true;
-      };
-      auto pv = [&](int m) -> bool {
-        const int n = m >> 1, h = m & 1, s = n & 1, i = 2 * pv_chunk + 1;
-        const uint32_t r = steps[n % kPgSteps];
-        if (!mbar_wait_bounded(b_p + 8 * (2 * s + h), (n >> 1) & 1)) return false;
-        if (h == 0 && !mbar_wait_bounded(b_full + 8 * (i % kRing), (i / kRing) & 1)) return false;
-        tc_fence_after();
-        const uint64_t vd = vdesc + ((s_ring + (i % kRing) * kTB + h * kPgHalf * 128) >> 4);
-        const uint32_t p = tmem + s * 128 + h * kPgHalf;
-        const bool fresh = (r & PgStep::kFirst) && h == 0;
+        for (int h = 0; h < 2; ++h) {
+          // the buffer is free once the product of two steps ago has read its probabilities
+          if (n >= 2 && !mbar_wait_bounded(b_pv + 8 * (2 * s + h), ((n >> 1) - 1) & 1)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < kPgHalf / 16; ++kk)
-          tc_mma_ta(tmem + kPgO + s * 128, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, !(fresh && kk == 0));
-        tc_commit(b_pv + 8 * (2 * s + h));
-        if (h == 1 && (r & PgStep::kRelease)) {
-          tc_commit(b_empty + 8 * (i % kRing));
-          ++pv_chunk;
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
+            tc_mma(tmem + s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+          }
+          tc_commit(b_s + 8 * (2 * s + h));
         }
-        return true;
-      };
-      for (int m = 0; m < 4 && !failed; ++m) failed = !qk(m);
-      for (int m = 0; !failed && (m >> 1) < last; ++m) failed = !pv(m) || !qk(m + 4);
+        if (failed) break;
+        if (rec & PgStep::kRelease) tc_commit(b_empty + 8 * r);
+        if (rec & PgStep::kQRelease) tc_commit(b_qempty + 8 * ((rec >> 8) & 15u));
+      }
       tc_commit(b_done);  // TMEM is freed only after every MMA has completed
+      mbar_wait_bounded(b_done, 0);
+    }
+  } else if (warp == kPgPvWarp) {
+    // ================================================================ O += P V (one lane)
+    if (lane == 0) {
+      constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc = pg_idesc(kFmt, D, true);
+      const uint64_t desc = tc_desc(0, kBox);
+      int r = 1, phase = 0;  // ring slot and phase parity of the step's V
+      for (int n = 0;; ++n) {
+        const int s = n & 1;
+        if (!mbar_wait_bounded(b_rec + 8 * (n & 3), (n >> 2) & 1)) {
+          failed = true;
+          break;
+        }
+        const uint32_t rec = steps[n % kPgSteps];
+        if (rec & PgStep::kStop) break;
+        if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
+          failed = true;
+          break;
+        }
+        const uint64_t vd = desc + ((s_ring + r * kTB) >> 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!mbar_wait_bounded(b_p + 8 * (2 * s + h), (n >> 1) & 1)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < kPgHalf / 16; ++kk)
+            tc_mma_ta(tmem + kPgO + s * 128, tmem + s * 128 + h * kPgHalf + kk * 8,
+                      vd + (4 * h + kk) * (2048 >> 4), idesc, h > 0 || kk > 0 || !(rec & PgStep::kFirst));
+          tc_commit(b_pv + 8 * (2 * s + h));
+        }
+        if (failed) break;
+        if (rec & PgStep::kRelease) {
+          tc_commit(b_empty + 8 * r);
+          if ((r += 2) >= kRing) {
+            r -= kRing;
+            phase ^= 1;
+          }
+        }
+      }
+      tc_commit(b_done);
       mbar_wait_bounded(b_done, 0);
     }
   } else {
@@ -790,7 +815,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         tc_fence_after();
         if (narrow) {
           // the four warps' results over their keys, joined in shared memory
-          float* part = reinterpret_cast<float*>(gbase + 2 * kTB + s * (G_::kMergeBytes / 2));  // [4][8][D]
+          float* part = reinterpret_cast<float*>(gbase + kTB + s * (G_::kMergeBytes / 2));  // [4][8][D]
           float2* ml = g_ml + s * 4 * kPgNarrow;
           if (lane < rows) ml[wq * kPgNarrow + lane] = make_float2(mref, l);
 #pragma unroll
