@@ -500,37 +500,59 @@ def raise_status(status: int) -> None:
                            "launches since the last check are void")
 
 
-def rotary(q: torch.Tensor, q_out: torch.Tensor, k: torch.Tensor | None, k_out: torch.Tensor | None,
-           positions: torch.Tensor, rot: Rotation) -> None:
-    """q_out = rotate(q) and k_out = rotate(k), [B, H, T, D] each, at positions [T] or [B, T]."""
-    stride_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    rc = lib().sink_rotary(q.shape[0], q.shape[3], ctypes.byref(rows_desc(q)), ctypes.byref(rows_desc(q_out)),
-                           ctypes.byref(rows_desc(k)) if k is not None else None,
-                           ctypes.byref(rows_desc(k_out)) if k is not None else None,
-                           positions.data_ptr(), stride_b, ctypes.byref(rot), stream_handle(q.device))
-    _check(rc, "sink_rotary")
+# Calls of these operators take a few microseconds on the GPU for a single token, so what a call
+# checks and describes is kept, per thread, under the shapes, strides, types and devices of its
+# arguments: a later call of the same form fills in addresses only.
+_thread = threading.local()
+_MAX_FORMS = 512
 
 
-def paged_append(kv: PagedKV, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None,
-                 q: torch.Tensor | None, q_out: torch.Tensor | None, rot: Rotation | None) -> None:
-    """The first counts[b] tokens of k, v [B, Hkv, T, D] into their pages (k rotated), q beside them."""
-    rc = lib().sink_paged_append(ctypes.byref(kv), ctypes.byref(rows_desc(k)), ctypes.byref(rows_desc(v)),
-                                 counts.data_ptr() if counts is not None else None,
-                                 ctypes.byref(rows_desc(q)) if q is not None else None,
-                                 ctypes.byref(rows_desc(q_out)) if q is not None else None,
-                                 ctypes.byref(rot) if rot is not None else None, stream_handle(k.device))
-    _check(rc, "sink_paged_append")
+def forms(kind: str) -> dict:
+    """This thread's descriptors of calls of `kind`, by form."""
+    d = _thread.__dict__.get(kind)
+    if d is None or len(d) > _MAX_FORMS:
+        d = _thread.__dict__[kind] = {}
+    return d
+
+
+def form_of(x: torch.Tensor | None):
+    """What a descriptor of `x` depends on, its address apart."""
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+
+
+class RowsArg:
+    """A sink_rows_t argument that is described once and pointed at a tensor per call."""
+
+    def __init__(self, t: torch.Tensor):
+        self.rows = rows_desc(t)
+        self.ref = ctypes.byref(self.rows)
+
+    def at(self, t: torch.Tensor):
+        self.rows.data = t.data_ptr()
+        return self.ref
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of device `index` as the C ABI takes it."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class on_device:
+    """Make device `index` current for the block; nothing to do when it is."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def paged_workspace_bytes(batch: int, heads_kv: int, heads_q: int, head_dim: int, shared_len: int,
                           num_sms: int) -> int:
     return int(lib().sink_paged_workspace_bytes(batch, heads_kv, heads_q, head_dim, shared_len, num_sms))
-
-
-def paged_attention(q: torch.Tensor, kv: PagedKV, shared_len: int, scale: float, out: torch.Tensor,
-                    workspace: torch.Tensor) -> None:
-    """out[B, 1, Hq, D] = attention of q [B, Hq, 1, D] over each sequence's rows [0, lens[b])."""
-    rc = lib().sink_paged_attention(ctypes.byref(rows_desc(q)), ctypes.byref(kv), shared_len, scale, out.data_ptr(),
-                                    out.stride(0), out.stride(2), workspace.data_ptr(), workspace.numel(),
-                                    stream_handle(q.device))
-    _check(rc, "sink_paged_attention")

@@ -291,9 +291,14 @@ __device__ __forceinline__ void pg_mask(uint32_t (&r)[N], int limit) {
 
 template <int N>
 __device__ __forceinline__ float pg_max(const uint32_t (&r)[N], float mx) {
+  float m[4] = {mx, kNegInf, kNegInf, kNegInf};  // four chains: latency, not rate, bounds a step
 #pragma unroll
-  for (int x = 0; x < N; ++x) mx = fmaxf(mx, __uint_as_float(r[x]));
-  return mx;
+  for (int x = 0; x < N; x += 8) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      m[y] = fmaxf(m[y], fmaxf(__uint_as_float(r[x + y]), __uint_as_float(r[x + 4 + y])));
+  }
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // Moves the row's reference maximum up to `mx` (log2 units) when that passes it by kPgRescale:
@@ -343,11 +348,10 @@ __device__ __forceinline__ void pg_probs(const uint32_t (&r)[N], uint64_t scale2
 
 // What the MMA warps have to know of a step, written by the load warp.
 struct PgStep {
-  static constexpr uint32_t kFirst = 1u, kLast = 2u;     // of the piece's steps on its stream
-  static constexpr uint32_t kRelease = 4u;               // the last step on its chunk
-  static constexpr uint32_t kQWait = 8u, kQRelease = 16u;// first, last use of the Q tile
-  static constexpr uint32_t kMore = 32u;                 // another step on the same chunk follows
-  static constexpr uint32_t kStop = 64u;                 // no step: the end
+  static constexpr uint32_t kFirst = 1u;                   // the piece's first step on its stream
+  static constexpr uint32_t kQWait = 2u, kQRelease = 4u;   // first, last chunk of the Q tile
+  static constexpr uint32_t kMore = 8u;                    // the chunk has a second step
+  static constexpr uint32_t kStop = 16u;                   // no step: the end
   // bits 8..11: Q slot (0, 1 wide; 2.. narrow), bit 12: the slot's phase parity, bits 16..: the
   // tile's shared-memory address in 16-byte words
 };
@@ -570,12 +574,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             if (v == 0) {  // the chunk's steps, published by the arrival
               const uint32_t ends = (j + 1 == pc.j1 ? PgStep::kQRelease : 0u) | (j == pc.j0 ? PgStep::kQWait : 0u);
               if (pc.pair) {
-                const uint32_t f = ends | (j == pc.j0 ? PgStep::kFirst : 0u) | (j + 1 == pc.j1 ? PgStep::kLast : 0u);
+                const uint32_t f = ends | (j == pc.j0 ? PgStep::kFirst : 0u);
                 steps[step % kPgSteps] = f | PgStep::kMore | q_bits[0];
-                steps[(step + 1) % kPgSteps] = f | PgStep::kRelease | q_bits[1];
+                steps[(step + 1) % kPgSteps] = f | q_bits[1];
               } else {
-                steps[step % kPgSteps] = ends | (j - pc.j0 < 2 ? PgStep::kFirst : 0u) |
-                                         (j + 2 >= pc.j1 ? PgStep::kLast : 0u) | PgStep::kRelease | q_bits[0];
+                steps[step % kPgSteps] = ends | (j - pc.j0 < 2 ? PgStep::kFirst : 0u) | q_bits[0];
               }
             }
             mbar_arrive_expect_tx(bar, kTB);
@@ -611,47 +614,51 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
       const uint64_t desc = tc_desc(0, 16);
-      uint32_t rec = 0;
-      int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest step's K
-      for (int n = 0;; ++n) {
-        const int s = n & 1;
-        if (!(rec & PgStep::kMore)) {  // a chunk of its own
-          if ((r += 2) >= kRing) {
-            r -= kRing;
-            phase ^= 1;
-          }
-          if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
-            failed = true;
-            break;
-          }
+      int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest K
+      for (int n = 0;;) {
+        if ((r += 2) >= kRing) {
+          r -= kRing;
+          phase ^= 1;
         }
-        rec = steps[n % kPgSteps];
-        mbar_arrive(b_rec + 8 * (n & 3));  // the P V warp may read it too
-        if (rec & PgStep::kStop) break;
-        if ((rec & PgStep::kQWait) && !mbar_wait_bounded(b_qfull + 8 * ((rec >> 8) & 15u), (rec >> 12) & 1u)) {
+        if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
           failed = true;
           break;
         }
-        const uint64_t qd = desc + (rec >> 16);
+        // a pair's chunk has two steps, whose halves take turns: both streams move on together
+        uint32_t rec[2];
+        rec[0] = rec[1] = steps[n % kPgSteps];
+        const int many = rec[0] & PgStep::kMore ? 2 : 1;
+        if (many == 2) rec[1] = steps[(n + 1) % kPgSteps];
+        for (int t = 0; t < many; ++t) mbar_arrive(b_rec + 8 * ((n + t) & 3));  // the P V warp may read them too
+        if (rec[0] & PgStep::kStop) break;
+        if (rec[0] & PgStep::kQWait)
+          for (int t = 0; t < many; ++t)
+            if (!mbar_wait_bounded(b_qfull + 8 * ((rec[t] >> 8) & 15u), (rec[t] >> 12) & 1u)) failed = true;
         const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          // the buffer is free once the product of two steps ago has read its probabilities
-          if (n >= 2 && !mbar_wait_bounded(b_pv + 8 * (2 * s + h), ((n >> 1) - 1) & 1)) {
-            failed = true;
-            break;
-          }
-          tc_fence_after();
+          for (int t = 0; t < many && !failed; ++t) {
+            const int s = (n + t) & 1;
+            // the buffer is free once the product of two steps ago has read its probabilities
+            if (n + t >= 2 && !mbar_wait_bounded(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t qd = desc + ((t ? rec[1] : rec[0]) >> 16);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
-            tc_mma(tmem + s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
+              tc_mma(tmem + s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+            }
+            tc_commit(b_s + 8 * (2 * s + h));
           }
-          tc_commit(b_s + 8 * (2 * s + h));
         }
         if (failed) break;
-        if (rec & PgStep::kRelease) tc_commit(b_empty + 8 * r);
-        if (rec & PgStep::kQRelease) tc_commit(b_qempty + 8 * ((rec >> 8) & 15u));
+        tc_commit(b_empty + 8 * r);
+        if (rec[0] & PgStep::kQRelease)
+          for (int t = 0; t < many; ++t) tc_commit(b_qempty + 8 * ((rec[t] >> 8) & 15u));
+        n += many;
       }
       tc_commit(b_done);  // TMEM is freed only after every MMA has completed
       mbar_wait_bounded(b_done, 0);
@@ -662,41 +669,45 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc = pg_idesc(kFmt, D, true);
       const uint64_t desc = tc_desc(0, kBox);
-      int r = 1, phase = 0;  // ring slot and phase parity of the step's V
-      for (int n = 0;; ++n) {
-        const int s = n & 1;
+      int r = 1, phase = 0;  // ring slot and phase parity of the chunk's V
+      for (int n = 0;;) {
         if (!mbar_wait_bounded(b_rec + 8 * (n & 3), (n >> 2) & 1)) {
           failed = true;
           break;
         }
-        const uint32_t rec = steps[n % kPgSteps];
+        const uint32_t rec = steps[n % kPgSteps];  // a pair's two steps are alike here
         if (rec & PgStep::kStop) break;
-        if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
+        const int many = rec & PgStep::kMore ? 2 : 1;
+        if (many == 2 && !mbar_wait_bounded(b_rec + 8 * ((n + 1) & 3), ((n + 1) >> 2) & 1)) failed = true;
+        if (failed || !mbar_wait_bounded(b_full + 8 * r, phase)) {
           failed = true;
           break;
         }
         const uint64_t vd = desc + ((s_ring + r * kTB) >> 4);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait_bounded(b_p + 8 * (2 * s + h), (n >> 1) & 1)) {
-            failed = true;
-            break;
-          }
-          tc_fence_after();
+          for (int t = 0; t < many; ++t) {
+            const int s = (n + t) & 1;
+            if (!mbar_wait_bounded(b_p + 8 * (2 * s + h), ((n + t) >> 1) & 1)) {
+              failed = true;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < kPgHalf / 16; ++kk)
-            tc_mma_ta(tmem + kPgO + s * 128, tmem + s * 128 + h * kPgHalf + kk * 8,
-                      vd + (4 * h + kk) * (2048 >> 4), idesc, h > 0 || kk > 0 || !(rec & PgStep::kFirst));
-          tc_commit(b_pv + 8 * (2 * s + h));
+            for (int kk = 0; kk < kPgHalf / 16; ++kk)
+              tc_mma_ta(tmem + kPgO + s * 128, tmem + s * 128 + h * kPgHalf + kk * 8,
+                        vd + (4 * h + kk) * (2048 >> 4), idesc, h > 0 || kk > 0 || !(rec & PgStep::kFirst));
+            tc_commit(b_pv + 8 * (2 * s + h));
+          }
+          if (failed) break;
         }
         if (failed) break;
-        if (rec & PgStep::kRelease) {
-          tc_commit(b_empty + 8 * r);
-          if ((r += 2) >= kRing) {
-            r -= kRing;
-            phase ^= 1;
-          }
+        tc_commit(b_empty + 8 * r);
+        if ((r += 2) >= kRing) {
+          r -= kRing;
+          phase ^= 1;
         }
+        n += many;
       }
       tc_commit(b_done);
       mbar_wait_bounded(b_done, 0);

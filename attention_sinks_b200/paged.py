@@ -23,7 +23,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .rope import _rotation, device_frequencies
+from .rope import device_frequencies, rotation
 
 # Scratch of `attend`, one buffer per (device, stream): calls on one stream run in order, so they
 # can share one.  Inside a graph capture a fresh one comes from the graph's own pool, so that
@@ -31,14 +31,50 @@ from .rope import _rotation, device_frequencies
 _SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+def _scratch(nbytes: int, index: int, stream: int) -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, _lib.stream_handle(device))
-    buf = _SCRATCH.get(key)
+        return torch.empty(nbytes, dtype=torch.uint8, device=index)
+    buf = _SCRATCH.get((index, stream))
     if buf is None or buf.numel() < nbytes:
-        buf = _SCRATCH[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf = _SCRATCH[index, stream] = torch.empty(nbytes, dtype=torch.uint8, device=index)
     return buf
+
+
+class _AppendCall:
+    """A checked form of `append` call, with the descriptors of its tensors."""
+
+    def __init__(self, cache, k, v, q, counts):
+        tokens = k.shape[2] if k.dim() == 4 else -1
+        self.copy = [False] * 3
+        for i, (name, x, heads) in enumerate((("k", k, cache.heads_kv), ("v", v, cache.heads_kv), ("q", q, None))):
+            if x is not None:
+                cache._check_rows(name, x, heads, tokens)
+                self.copy[i] = x.stride(-1) != 1
+        if counts is not None and (counts.shape != (cache.batch,) or counts.dtype != torch.int32
+                                   or counts.device != cache.device or not counts.is_contiguous()):
+            raise ValueError(f"counts is a contiguous int32 [{cache.batch}] tensor on {cache.device}")
+        self.empty = not (tokens and cache.batch)
+        k, v, q = (x if x is None else x.detach().contiguous() if c else x.detach()
+                   for x, c in zip((k, v, q), self.copy))
+        self.k, self.v = _lib.RowsArg(k), _lib.RowsArg(v)
+        if q is not None:
+            self.q, self.q_out = _lib.RowsArg(q), _lib.RowsArg(torch.empty_like(q))
+
+
+class _AttendCall:
+    """A checked form of `attend` call."""
+
+    def __init__(self, cache, q, shared_len, aligned):
+        cache._check_rows("q", q, None, 1)
+        b, hq, _, d = q.shape
+        # the kernel's tiled copies start rows on 16-byte boundaries
+        self.copy = (not aligned or q.stride(-1) != 1 or q.stride(0) % 8 or q.stride(1) % 8
+                     or min(q.stride(0), q.stride(1)) < d)
+        self.shape = (b, 1, hq, d)
+        self.q = _lib.RowsArg(q.detach().clone(memory_format=torch.contiguous_format) if self.copy else q.detach())
+        # shapes that the kernel refuses need nothing: the call says why
+        self.workspace = max(256, _lib.paged_workspace_bytes(b, cache.heads_kv, hq, d, shared_len,
+                                                             _lib.sm_count(cache.device)))
 
 
 class PagedKVCache:
@@ -85,23 +121,28 @@ class PagedKVCache:
         self.device, self.dtype = device, k_pages.dtype
         self.batch, self.heads_kv, self.page_size, self.head_dim = batch, hkv, page, d
         self.inv_freq = None if inv_freq is None else device_frequencies(inv_freq, device)
-        self._rot = None if inv_freq is None else _rotation(self.inv_freq, interleaved, attention_scaling, False)
+        rot = None if inv_freq is None else rotation(self.inv_freq, interleaved, attention_scaling)
         self._kv = _lib.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lens.data_ptr(),
                                 status.data_ptr(), _lib.dtype_code(k_pages.dtype), batch, hkv, d, page, pages, width, 0,
                                 block_table.stride(0), k_pages.stride(0), k_pages.stride(1), v_pages.stride(0),
                                 v_pages.stride(1))
+        self._rot = rot
+        self._kv_ref, self._rot_ref = ctypes.byref(self._kv), None if rot is None else ctypes.byref(rot)
+        self._index = device.index
         _lib.prepare_device(device)  # before any graph capture of this cache's steps
+        self._like = (k_pages.dtype, batch, hkv, d, device)  # what a call's form depends on here
 
-    def _rows(self, name: str, x: torch.Tensor, heads: int | None, tokens: int) -> torch.Tensor:
-        """x as the kernels take it, [B, heads, tokens, D] with a unit last stride."""
+    def _check_rows(self, name: str, x: torch.Tensor, heads: int | None, tokens: int) -> None:
         if (x.dim() != 4 or x.shape[0] != self.batch or (heads is not None and x.shape[1] != heads)
                 or x.shape[2] != tokens or x.shape[3] != self.head_dim or x.dtype != self.dtype
                 or x.device != self.device):
             raise ValueError(f"{name} is [{self.batch}, {heads or 'Hq'}, {tokens}, {self.head_dim}] {self.dtype} on "
                              f"{self.device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"the paged cache keeps no gradients: call it under torch.no_grad() or detach {name}")
-        return x if x.stride(-1) == 1 else x.contiguous()
+
+    @staticmethod
+    def _no_gradients(*tensors: torch.Tensor | None) -> None:
+        if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+            raise RuntimeError("the paged cache keeps no gradients: call it under torch.no_grad() or detach its inputs")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                counts: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -110,18 +151,25 @@ class PagedKVCache:
         positions.  Returns q [B, Hq, T, D] rotated to them too, in one launch (None without q).
         Tokens from counts[b] on, and all of an idle sequence's (lens 0), are not stored; their
         q rows come back as zeros.  counts: int32 [B] on the device."""
-        tokens = k.shape[2] if k.dim() == 4 else -1
-        k, v = self._rows("k", k, self.heads_kv, tokens), self._rows("v", v, self.heads_kv, tokens)
-        if counts is not None and (counts.shape != (self.batch,) or counts.dtype != torch.int32
-                                   or counts.device != self.device or not counts.is_contiguous()):
-            raise ValueError(f"counts is a contiguous int32 [{self.batch}] tensor on {self.device}")
-        q_out = None
-        if q is not None:
-            q = self._rows("q", q, None, tokens)
-            q_out = torch.empty_like(q)
-        if tokens and self.batch:
-            with torch.cuda.device(self.device):
-                _lib.paged_append(self._kv, k, v, counts, q, q_out, self._rot)
+        self._no_gradients(k, v, q)
+        form = (self._like, _lib.form_of(k), _lib.form_of(v), _lib.form_of(q), _lib.form_of(counts))
+        known = _lib.forms("append")
+        call = known.get(form)
+        if call is None:
+            call = known[form] = _AppendCall(self, k, v, q, counts)
+        if any(call.copy):
+            k, v, q = (x.contiguous() if c else x for x, c in zip((k, v, q), call.copy))
+        q_out = None if q is None else torch.empty_like(q)
+        if call.empty:
+            return q_out
+        with _lib.on_device(self._index):
+            rc = _lib.lib().sink_paged_append(self._kv_ref, call.k.at(k), call.v.at(v),
+                                              None if counts is None else counts.data_ptr(),
+                                              None if q is None else call.q.at(q),
+                                              None if q is None else call.q_out.at(q_out), self._rot_ref,
+                                              _lib.raw_stream(self._index))
+        if rc:
+            _lib._check(rc, "sink_paged_append")
         return q_out
 
     def attend(self, q: torch.Tensor, scale: float | None = None, shared_len: int = 0) -> torch.Tensor:
@@ -133,24 +181,34 @@ class PagedKVCache:
         sequences: they are read through the first row of the block table, once per kv head
         for the whole batch.  bfloat16 or float16, head_dim 64 or 128, pages of 16, 32, 64 or
         128 rows, up to 8 query heads per kv head."""
-        q = self._rows("q", q, None, 1)
-        b, hq, _, d = q.shape
-        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8 or min(q.stride(0), q.stride(1)) < d:
-            q = q.contiguous()  # the kernel's tiled copies start rows on 16-byte boundaries
-        out = torch.empty(b, 1, hq, d, dtype=q.dtype, device=self.device)
-        if b == 0:
+        self._no_gradients(q)
+        aligned = q.data_ptr() % 16 == 0
+        form = (self._like, _lib.form_of(q), shared_len, aligned)
+        known = _lib.forms("attend")
+        call = known.get(form)
+        if call is None:
+            call = known[form] = _AttendCall(self, q, shared_len, aligned)
+        if call.copy:
+            q = q.clone(memory_format=torch.contiguous_format)
+        out = torch.empty(call.shape, dtype=self.dtype, device=self._index)
+        if self.batch == 0:
             return out
-        need = _lib.paged_workspace_bytes(b, self.heads_kv, hq, d, shared_len, _lib.sm_count(self.device))
-        with torch.cuda.device(self.device):
-            _lib.paged_attention(q, self._kv, shared_len, d ** -0.5 if scale is None else scale, out,
-                                 _scratch(max(need, 256), self.device))
+        with _lib.on_device(self._index):
+            stream = _lib.raw_stream(self._index)
+            work = _scratch(call.workspace, self._index, stream)
+            rc = _lib.lib().sink_paged_attention(call.q.at(q), self._kv_ref, shared_len,
+                                                 self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                                                 call.shape[2] * self.head_dim, self.head_dim, work.data_ptr(),
+                                                 work.numel(), stream)
+        if rc:
+            _lib._check(rc, "sink_paged_attention")
         return out
 
     def check_status(self) -> None:
         """Raise RuntimeError if a kernel met a position past the block table or a page outside
         the pool since the last check (nothing was accessed there); synchronises the stream."""
         st = ctypes.c_int32(0)
-        with torch.cuda.device(self.device):
-            _lib._check(_lib.lib().sink_read_status(self.status.data_ptr(), _lib.stream_handle(self.device),
+        with _lib.on_device(self._index):
+            _lib._check(_lib.lib().sink_read_status(self.status.data_ptr(), _lib.raw_stream(self._index),
                                                     ctypes.byref(st)), "sink_read_status")
         _lib.raise_status(st.value)

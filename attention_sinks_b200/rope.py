@@ -16,6 +16,7 @@ pairs, a part of the head, fp64 angles, with its backward pass.  `rope_frequenci
 frequencies it takes, scaled for long contexts where asked.
 """
 
+import ctypes
 import math
 
 import torch
@@ -112,7 +113,7 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, kind: str = "default",
     raise ValueError(f"unknown kind of frequency scaling {kind!r}")
 
 
-def _rotation(inv_freq: torch.Tensor, interleaved: bool, scale: float, inverse: bool) -> "_lib.Rotation":
+def rotation(inv_freq: torch.Tensor, interleaved: bool, scale: float, inverse: bool = False) -> "_lib.Rotation":
     return _lib.Rotation(inv_freq.data_ptr(), inv_freq.numel(), int(interleaved), float(scale), int(inverse))
 
 
@@ -123,19 +124,76 @@ def device_frequencies(inv_freq: torch.Tensor, device: torch.device) -> torch.Te
     return inv_freq.detach().to(device, torch.float64).contiguous()
 
 
+class _RotaryCall:
+    """A checked form of `rotary` call, with the descriptors of its tensors."""
+
+    def __init__(self, q, k, positions, inv_freq):
+        if q.dim() != 4:
+            raise ValueError(f"q is [B, H, T, D], got {tuple(q.shape)}")
+        device = q.device
+        _lib.check_device(device)
+        _lib.dtype_code(q.dtype)
+        b, _, t, d = q.shape
+        if k is not None and (k.dim() != 4 or k.shape[0] != b or k.shape[2] != t or k.shape[3] != d
+                              or k.dtype != q.dtype or k.device != device):
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} {k.device} does not go with q {tuple(q.shape)} {q.dtype} "
+                             f"{device}")
+        if positions.device != device or positions.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"positions are whole numbers on {device}, got {positions.dtype} on {positions.device}")
+        if positions.shape not in ((t,), (b, t), (1, t)):
+            raise ValueError(f"positions are [{t}] or [{b}, {t}], got {tuple(positions.shape)}")
+        if 2 * inv_freq.numel() > d or d > 512:
+            raise ValueError(f"{2 * inv_freq.numel()} rotated dims of a head of {d} (at most 512)")
+        self.device, self.index = device, device.index
+        self.batch, self.dim = b, d
+        # what a call has to convert first
+        self.copy_q = q.stride(-1) != 1
+        self.copy_k = k is not None and k.stride(-1) != 1
+        self.copy_positions = positions.dtype != torch.int64 or (t > 1 and positions.stride(-1) != 1)
+        self.copy_freq = inv_freq.dtype != torch.float64 or inv_freq.device != device or not inv_freq.is_contiguous()
+        self.empty = not (q.numel() or (k is not None and k.numel()))
+        q = q.detach().contiguous() if self.copy_q else q.detach()
+        self.q, self.q_out = _lib.RowsArg(q), _lib.RowsArg(torch.empty_like(q))
+        if k is not None:
+            k = k.detach().contiguous() if self.copy_k else k.detach()
+            self.k, self.k_out = _lib.RowsArg(k), _lib.RowsArg(torch.empty_like(k))
+        several = positions.dim() == 2 and positions.shape[0] > 1
+        self.pos_stride = 0 if not several else t if self.copy_positions else positions.stride(0)
+        self.rot = _lib.Rotation(0, inv_freq.numel(), 0, 1.0, 0)
+        self.rot_ref = ctypes.byref(self.rot)
+
+    def __call__(self, q, k, positions, inv_freq, interleaved, scale, inverse):
+        if self.copy_q:
+            q = q.contiguous()
+        if self.copy_k:
+            k = k.contiguous()
+        q_out = torch.empty_like(q)
+        k_out = None if k is None else torch.empty_like(k)
+        if self.empty:
+            return q_out, k_out
+        if self.copy_positions:
+            positions = positions.to(torch.int64).contiguous()
+        if self.copy_freq:
+            inv_freq = device_frequencies(inv_freq, self.device)
+        rot = self.rot
+        rot.inv_freq, rot.interleaved, rot.scale, rot.inverse = inv_freq.data_ptr(), interleaved, scale, inverse
+        with _lib.on_device(self.index):
+            rc = _lib.lib().sink_rotary(self.batch, self.dim, self.q.at(q), self.q_out.at(q_out),
+                                        None if k is None else self.k.at(k),
+                                        None if k is None else self.k_out.at(k_out), positions.data_ptr(),
+                                        self.pos_stride, self.rot_ref, _lib.raw_stream(self.index))
+        if rc:
+            _lib._check(rc, "sink_rotary")
+        return q_out, k_out
+
+
 def _launch(q, k, positions, inv_freq, interleaved, scale, inverse):
-    outs = []
-    ins = []
-    for x in (q, k):
-        if x is not None and x.stride(-1) != 1:
-            x = x.contiguous()
-        ins.append(x)
-        outs.append(torch.empty_like(x) if x is not None else None)
-    if q.numel() or (k is not None and k.numel()):
-        with torch.cuda.device(q.device):
-            _lib.rotary(ins[0], outs[0], ins[1], outs[1], positions,
-                        _rotation(inv_freq, interleaved, scale, inverse))
-    return outs[0], outs[1]
+    form = (_lib.form_of(q), _lib.form_of(k), _lib.form_of(positions), _lib.form_of(inv_freq))
+    known = _lib.forms("rotary")
+    call = known.get(form)
+    if call is None:
+        call = known[form] = _RotaryCall(q, k, positions, inv_freq)
+    return call(q, k, positions, inv_freq, interleaved, scale, inverse)
 
 
 class _Rotary(torch.autograd.Function):
@@ -182,25 +240,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     Forward and backward can be captured into a CUDA graph, on torch's terms: no autograd graph
     of the same leaf tensors made outside the capture may be alive.
     """
-    if q.dim() != 4:
-        raise ValueError(f"q is [B, H, T, D], got {tuple(q.shape)}")
-    device = q.device
-    _lib.check_device(device)
-    _lib.dtype_code(q.dtype)
-    b, _, t, d = q.shape
-    if k is not None and (k.dim() != 4 or k.shape[0] != b or k.shape[2] != t or k.shape[3] != d
-                          or k.dtype != q.dtype or k.device != device):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} {k.device} does not go with q {tuple(q.shape)} {q.dtype} "
-                         f"{device}")
-    if positions.device != device or positions.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"positions are whole numbers on {device}, got {positions.dtype} on {positions.device}")
-    if positions.shape not in ((t,), (b, t), (1, t)):
-        raise ValueError(f"positions are [{t}] or [{b}, {t}], got {tuple(positions.shape)}")
-    if 2 * inv_freq.numel() > d or d > 512:
-        raise ValueError(f"{2 * inv_freq.numel()} rotated dims of a head of {d} (at most 512)")
-    if positions.dtype != torch.int64 or (t > 1 and positions.stride(-1) != 1):
-        positions = positions.to(torch.int64).contiguous()
-    inv_freq = device_frequencies(inv_freq, device)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = _Rotary.apply(q, k, positions, inv_freq, interleaved, attention_scaling, False)
         return out if k is not None else (out, None)
