@@ -99,10 +99,10 @@ struct PagedArgs {
 // time that memory takes for all of it (kOwnMem when every SM streams).
 template <int D>
 struct PgCost {
-  static constexpr int kPair = D == 128 ? 40 : 38;
-  static constexpr int kOne = D == 128 ? 24 : 22;
-  static constexpr int kOwnMin = D == 128 ? 20 : 16;
-  static constexpr int kOwnMem = D == 128 ? 43 : 22;
+  static constexpr int kPair = D == 128 ? 76 : 62;
+  static constexpr int kOne = D == 128 ? 38 : 32;
+  static constexpr int kOwnMin = D == 128 ? 34 : 27;
+  static constexpr int kOwnMem = D == 128 ? 43 : 28;
 };
 
 struct PagedLine {
@@ -239,6 +239,17 @@ __device__ __forceinline__ float pg_exp2(float x) {
   return y;
 }
 
+// True in one lane of the warp.
+__device__ __forceinline__ bool pg_elect() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // A bounded wait whose answer the whole warp shares.
 __device__ __forceinline__ bool pg_warp_wait(uint32_t bar, uint32_t parity) {
   return __all_sync(kFull, mbar_wait_bounded(bar, parity));
@@ -290,8 +301,8 @@ __device__ __forceinline__ void pg_mask(uint32_t (&r)[N], int limit) {
 }
 
 template <int N>
-__device__ __forceinline__ float pg_max(const uint32_t (&r)[N], float mx) {
-  float m[4] = {mx, kNegInf, kNegInf, kNegInf};  // four chains: latency, not rate, bounds a step
+__device__ __forceinline__ float pg_max(const uint32_t (&r)[N]) {
+  float m[4] = {kNegInf, kNegInf, kNegInf, kNegInf};  // four chains: latency, not rate, bounds a step
 #pragma unroll
   for (int x = 0; x < N; x += 8) {
 #pragma unroll
@@ -333,17 +344,43 @@ __device__ __forceinline__ bool pg_reference(float mx, bool valid, bool has_o, u
 }
 
 // Probabilities 2^(scale s - m) of N scores, their sum added to `sum` (two accumulators),
-// rounded to T and packed.
+// rounded to T and packed.  (Half, a quarter or an eighth of the powers in FMA arithmetic beside
+// the special-function unit changed nothing: 256 query rows x 32K keys 141 us each way.)
 template <typename T, int N>
-__device__ __forceinline__ void pg_probs(const uint32_t (&r)[N], uint64_t scale2, uint64_t m2, uint64_t (&sum)[2],
+__device__ __forceinline__ void pg_probs(const uint32_t (&r)[N], uint64_t scale2, float m, uint64_t (&sum)[2],
                                          uint32_t* pk) {
+  const uint64_t m2 = pg_pair(-m, -m);
 #pragma unroll
   for (int x = 0; x < N / 2; ++x) {
-    const float2 e = pg_two(pg_fma2(pg_pair(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), scale2, m2));
-    const float p0 = pg_exp2(e.x), p1 = pg_exp2(e.y);
+    const uint64_t e = pg_fma2(pg_pair(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1])), scale2, m2);
+    const float2 v = pg_two(e);
+    const float p0 = pg_exp2(v.x), p1 = pg_exp2(v.y);
     sum[x & 1] = pg_add2(sum[x & 1], pg_pair(p0, p1));
     pk[x] = pg_pack<T>(p0, p1);
   }
+}
+
+// The softmax of a half step on N scores of the thread's row: packed probabilities, and l, mref
+// and O moved on.  The probabilities are taken against the reference maximum as it stands while
+// the scores' own maximum is still being found, so that neither waits for the other, and
+// taken again in the rare half step that moves the reference; a piece's first half step
+// (`fresh`) knows no reference yet and looks first.  False when a wait ran out.
+template <typename T, int D, int N>
+__device__ __forceinline__ bool pg_half_step(uint32_t (&r)[N], int keys, bool valid, bool fresh, float scale,
+                                             uint64_t scale2, uint32_t t_o, uint32_t b_pv, uint32_t parity,
+                                             float& mref, float& l, uint32_t* pk) {
+  pg_mask(r, keys);
+  uint64_t sum[2] = {0, 0};
+  if (!fresh) pg_probs<T>(r, scale2, mref == kNegInf ? 0.f : mref, sum, pk);
+  const float mx = pg_max(r) * scale;
+  if (__any_sync(kFull, valid && mx > mref + kPgRescale) || fresh) {
+    if (!pg_reference<D>(mx, valid, !fresh, t_o, b_pv, parity, mref, l)) return false;
+    sum[0] = sum[1] = 0;
+    pg_probs<T>(r, scale2, mref == kNegInf ? 0.f : mref, sum, pk);
+  }
+  const float2 add = pg_two(pg_add2(sum[0], sum[1]));
+  l += add.x + add.y;
+  return true;
 }
 
 // What the MMA warps have to know of a step, written by the load warp.
@@ -469,7 +506,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;  // the CTA holds all 512 columns
+  const uint32_t tmem_held = *tmem_slot;
   if (walk.lo < L.prefix_cost) {
     walk.own = false;
     walk.len = 0;
@@ -609,109 +647,124 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       for (int i = thin - 1; i >= 0 && i >= thin - 4; --i) pg_warp_wait(b_qfull + 8 * (2 + (i & 3)), (i >> 2) & 1);
     }
   } else if (warp == kPgQkWarp) {
-    // ================================================================ S = Q K^T (one lane)
-    if (lane == 0) {
-      constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
-      const uint64_t desc = tc_desc(0, 16);
-      int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest K
-      for (int n = 0;;) {
-        if ((r += 2) >= kRing) {
-          r -= kRing;
-          phase ^= 1;
-        }
-        if (!mbar_wait_bounded(b_full + 8 * r, phase)) {
-          failed = true;
-          break;
-        }
-        // a pair's chunk has two steps, whose halves take turns: both streams move on together
-        uint32_t rec[2];
-        rec[0] = rec[1] = steps[n % kPgSteps];
-        const int many = rec[0] & PgStep::kMore ? 2 : 1;
-        if (many == 2) rec[1] = steps[(n + 1) % kPgSteps];
+    // ================================================================ S = Q K^T
+    // The MMA warps run as whole warps and let one lane issue: their addresses and descriptors
+    // are then the same in every lane for the compiler too, and stay in uniform registers (issued
+    // from inside a one-lane branch an MMA took 57 clocks, 30 this way).
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
+    const uint64_t desc = tc_desc(0, 16);
+    const bool leader = pg_elect();
+    int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest K
+    for (int n = 0;;) {
+      if ((r += 2) >= kRing) {
+        r -= kRing;
+        phase ^= 1;
+      }
+      if (!pg_warp_wait(b_full + 8 * r, phase)) {
+        failed = true;
+        break;
+      }
+      // a pair's chunk has two steps, whose halves take turns: both streams move on together
+      const uint32_t rec = steps[n % kPgSteps];
+      const int many = rec & PgStep::kMore ? 2 : 1;
+      const uint32_t rec1 = many == 2 ? steps[(n + 1) % kPgSteps] : rec;
+      if (leader)
         for (int t = 0; t < many; ++t) mbar_arrive(b_rec + 8 * ((n + t) & 3));  // the P V warp may read them too
-        if (rec[0] & PgStep::kStop) break;
-        if (rec[0] & PgStep::kQWait)
-          for (int t = 0; t < many; ++t)
-            if (!mbar_wait_bounded(b_qfull + 8 * ((rec[t] >> 8) & 15u), (rec[t] >> 12) & 1u)) failed = true;
-        const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
+      if (rec & PgStep::kStop) break;
+      if (rec & PgStep::kQWait) {
+        if (!pg_warp_wait(b_qfull + 8 * ((rec >> 8) & 15u), (rec >> 12) & 1u)) failed = true;
+        if (many == 2 && !pg_warp_wait(b_qfull + 8 * ((rec1 >> 8) & 15u), (rec1 >> 12) & 1u)) failed = true;
+        if (failed) break;
+      }
+      const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          for (int t = 0; t < many && !failed; ++t) {
-            const int s = (n + t) & 1;
-            // the buffer is free once the product of two steps ago has read its probabilities
-            if (n + t >= 2 && !mbar_wait_bounded(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
-              failed = true;
-              break;
-            }
-            tc_fence_after();
-            const uint64_t qd = desc + ((t ? rec[1] : rec[0]) >> 16);
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+        for (int t = 0; t < many; ++t) {
+          const int s = (n + t) & 1;
+          // the buffer is free once the product of two steps ago has read its probabilities
+          if (n + t >= 2 && !pg_warp_wait(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t qd = desc + ((t ? rec1 : rec) >> 16);
+          if (leader) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
-              tc_mma(tmem + s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+              tc_mma(s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
             }
             tc_commit(b_s + 8 * (2 * s + h));
           }
         }
         if (failed) break;
-        tc_commit(b_empty + 8 * r);
-        if (rec[0] & PgStep::kQRelease)
-          for (int t = 0; t < many; ++t) tc_commit(b_qempty + 8 * ((rec[t] >> 8) & 15u));
-        n += many;
       }
-      tc_commit(b_done);  // TMEM is freed only after every MMA has completed
-      mbar_wait_bounded(b_done, 0);
+      if (failed) break;
+      if (leader) {
+        tc_commit(b_empty + 8 * r);
+        if (rec & PgStep::kQRelease) {
+          tc_commit(b_qempty + 8 * ((rec >> 8) & 15u));
+          if (many == 2) tc_commit(b_qempty + 8 * ((rec1 >> 8) & 15u));
+        }
+      }
+      n += many;
     }
+    if (leader) tc_commit(b_done);  // TMEM is freed only after every MMA has completed
+    pg_warp_wait(b_done, 0);
   } else if (warp == kPgPvWarp) {
-    // ================================================================ O += P V (one lane)
-    if (lane == 0) {
-      constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t idesc = pg_idesc(kFmt, D, true);
-      const uint64_t desc = tc_desc(0, kBox);
-      int r = 1, phase = 0;  // ring slot and phase parity of the chunk's V
-      for (int n = 0;;) {
-        if (!mbar_wait_bounded(b_rec + 8 * (n & 3), (n >> 2) & 1)) {
-          failed = true;
-          break;
-        }
-        const uint32_t rec = steps[n % kPgSteps];  // a pair's two steps are alike here
-        if (rec & PgStep::kStop) break;
-        const int many = rec & PgStep::kMore ? 2 : 1;
-        if (many == 2 && !mbar_wait_bounded(b_rec + 8 * ((n + 1) & 3), ((n + 1) >> 2) & 1)) failed = true;
-        if (failed || !mbar_wait_bounded(b_full + 8 * r, phase)) {
-          failed = true;
-          break;
-        }
-        const uint64_t vd = desc + ((s_ring + r * kTB) >> 4);
+    // ================================================================ O += P V
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t idesc = pg_idesc(kFmt, D, true);
+    const uint64_t desc = tc_desc(0, kBox);
+    const bool leader = pg_elect();
+    int r = 1, phase = 0;  // ring slot and phase parity of the chunk's V
+    for (int n = 0;;) {
+      if (!pg_warp_wait(b_rec + 8 * (n & 3), (n >> 2) & 1)) {
+        failed = true;
+        break;
+      }
+      const uint32_t rec = steps[n % kPgSteps];  // a pair's two steps are alike here
+      if (rec & PgStep::kStop) break;
+      const int many = rec & PgStep::kMore ? 2 : 1;
+      if (many == 2 && !pg_warp_wait(b_rec + 8 * ((n + 1) & 3), ((n + 1) >> 2) & 1)) failed = true;
+      if (failed || !pg_warp_wait(b_full + 8 * r, phase)) {
+        failed = true;
+        break;
+      }
+      const uint64_t vd = desc + ((s_ring + r * kTB) >> 4);
+      const bool first = rec & PgStep::kFirst;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          for (int t = 0; t < many; ++t) {
-            const int s = (n + t) & 1;
-            if (!mbar_wait_bounded(b_p + 8 * (2 * s + h), ((n + t) >> 1) & 1)) {
-              failed = true;
-              break;
-            }
-            tc_fence_after();
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+        for (int t = 0; t < many; ++t) {
+          const int s = (n + t) & 1;
+          if (!pg_warp_wait(b_p + 8 * (2 * s + h), ((n + t) >> 1) & 1)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          if (leader) {
 #pragma unroll
             for (int kk = 0; kk < kPgHalf / 16; ++kk)
-              tc_mma_ta(tmem + kPgO + s * 128, tmem + s * 128 + h * kPgHalf + kk * 8,
-                        vd + (4 * h + kk) * (2048 >> 4), idesc, h > 0 || kk > 0 || !(rec & PgStep::kFirst));
+              tc_mma_ta(kPgO + s * 128, s * 128 + h * kPgHalf + kk * 8, vd + (4 * h + kk) * (2048 >> 4), idesc,
+                        h > 0 || kk > 0 || !first);
             tc_commit(b_pv + 8 * (2 * s + h));
           }
-          if (failed) break;
         }
         if (failed) break;
-        tc_commit(b_empty + 8 * r);
-        if ((r += 2) >= kRing) {
-          r -= kRing;
-          phase ^= 1;
-        }
-        n += many;
       }
-      tc_commit(b_done);
-      mbar_wait_bounded(b_done, 0);
+      if (failed) break;
+      if (leader) tc_commit(b_empty + 8 * r);
+      if ((r += 2) >= kRing) {
+        r -= kRing;
+        phase ^= 1;
+      }
+      n += many;
     }
+    if (leader) tc_commit(b_done);
+    pg_warp_wait(b_done, 0);
   } else {
     // ================================================================ softmax: warpgroup s, a thread per query row
     const int s = warp >> 2, row = tid & 127, wq = warp & 3;
@@ -739,79 +792,80 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       for (int c = pc.pair ? 0 : t; c < n && !failed; c += inc) {
         const int st = pc.pair ? step + 2 * c + t : step + c;
         const int limit = end - (pc.j0 + c) * kPgKeys;  // keys of this chunk that count
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int keys = limit - h * kPgHalf;
-          const uint32_t t_h = t_s + h * kPgHalf;  // the half's scores, and P over their first 32 columns
-          const bool has_o = c >= inc || h == 1;
-          // the half step before on this stream: its P V is complete before O may be rescaled
-          const uint32_t b_before = b_pv + 8 * (2 * s + (h ^ 1)), p_before = ((st >> 1) - (h ^ 1)) & 1;
-          if (!pg_warp_wait(b_s + 8 * (2 * s + h), (st >> 1) & 1)) {
+        const uint32_t phase = (st >> 1) & 1;
+        if (!pg_warp_wait(b_s + 16 * s, phase)) {
+          failed = true;
+          break;
+        }
+        if (limit < kPgKeys && limit % A.page_size != 0) {
+          // The last page's rows past the end hold anything: zeros instead, so that their
+          // probability of 0 gives 0.  (This step's scores are there, so the slot's tile before has
+          // been read and the barrier is in this tile's phase.)
+          const int i = 2 * (chunk + c) + 1;
+          if (!pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1)) {
             failed = true;
             break;
           }
-          if (h == 0 && limit < kPgKeys && limit % A.page_size != 0) {
-            // The last page's rows past the end hold anything: zeros instead, so that their
-            // probability of 0 gives 0.  (This step's scores are there, so the slot's tile before
-            // has been read and the barrier is in this tile's phase.)
-            const int i = 2 * (chunk + c) + 1;
-            if (!pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1)) {
+          const int stop = (limit / A.page_size + 1) * A.page_size;
+          unsigned char* vt = gbase + (s_ring - base) + (i % kRing) * kTB;
+          for (int x = row; x < (stop - limit) * kBoxes * 8; x += 128) {
+            const int box = x / ((stop - limit) * 8), r = x - box * (stop - limit) * 8;
+            *reinterpret_cast<uint4*>(vt + box * kBox + limit * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        if (narrow) {  // both halves at once: a warp's keys are in one of them
+          if (!pg_warp_wait(b_s + 16 * s + 8, phase)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          uint32_t r[32], pk[16], none[16];
+          tc_ld_raw(t_s + 32 * wq, r);
+          tc_wait_ld();
+          // (the product before is complete: the second half's scores were issued after it)
+          if (!pg_half_step<T, D>(r, limit - 32 * wq, lane < rows, c < inc, A.scale_log2, scale2, t_o, b_pv + 16 * s + 8,
+                                  phase ^ 1, mref, l, pk)) {
+            failed = true;
+            break;
+          }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) none[x] = 0u;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // no probability for the other warps' keys
+            if (x == wq)
+              tc_st_raw(t_s + (x >> 1) * kPgHalf + (x & 1) * 16, pk);
+            else
+              tc_st_raw(t_s + (x >> 1) * kPgHalf + (x & 1) * 16, none);
+          }
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(b_p + 16 * s);
+          mbar_arrive(b_p + 16 * s + 8);
+          continue;
+        }
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !pg_warp_wait(b_s + 16 * s + 8, phase)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          if (!idle) {
+            uint32_t r[64], pk[32];
+            tc_ld_raw(t_s + h * kPgHalf, r);
+            tc_wait_ld();
+            // the half step before on this stream: its product is complete before O may be rescaled
+            if (!pg_half_step<T, D>(r, limit - h * kPgHalf, row < rows, c < inc && h == 0, A.scale_log2, scale2, t_o,
+                                    b_pv + 16 * s + 8 * (h ^ 1), phase ^ h ^ 1, mref, l, pk)) {
               failed = true;
               break;
             }
-            const int stop = (limit / A.page_size + 1) * A.page_size;
-            unsigned char* vt = gbase + (s_ring - base) + (i % kRing) * kTB;
-            for (int x = row; x < (stop - limit) * kBoxes * 8; x += 128) {
-              const int box = x / ((stop - limit) * 8), r = x - box * (stop - limit) * 8;
-              *reinterpret_cast<uint4*>(vt + box * kBox + limit * 128 + r * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
+            tc_st_raw(t_s + h * kPgHalf, pk);  // over the half's own scores
+            tc_wait_st();
           }
-          tc_fence_after();
-          uint64_t sum[2] = {0, 0};
-          bool ok = true;
-          if (narrow) {
-            uint32_t r[16], pk[8], none[8];
-            tc_ld_raw(t_h + 16 * wq, r);
-            tc_wait_ld();
-            pg_mask(r, keys - 16 * wq);
-            ok = pg_reference<D>(pg_max(r, kNegInf) * A.scale_log2, lane < rows, has_o, t_o, b_before, p_before, mref,
-                                 l);
-            const float m = mref == kNegInf ? 0.f : -mref;
-            pg_probs<T>(r, scale2, pg_pair(m, m), sum, pk);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) none[x] = 0u;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {  // no probability for the other warps' keys
-              if (x == wq)
-                tc_st_raw(t_h + 8 * x, pk);
-              else
-                tc_st_raw(t_h + 8 * x, none);
-            }
-          } else if (!idle) {
-            uint32_t x0[32], x1[32], pk[32];
-            tc_ld_raw(t_h, x0);
-            tc_ld_raw(t_h + 32, x1);
-            tc_wait_ld();
-            pg_mask(x0, keys);
-            pg_mask(x1, keys - 32);
-            ok = pg_reference<D>(pg_max(x1, pg_max(x0, kNegInf)) * A.scale_log2, row < rows, has_o, t_o, b_before,
-                                 p_before, mref, l);
-            const float m = mref == kNegInf ? 0.f : -mref;
-            const uint64_t m2 = pg_pair(m, m);
-            pg_probs<T>(x0, scale2, m2, sum, pk);
-            pg_probs<T>(x1, scale2, m2, sum, pk + 16);
-            tc_st_raw(t_h, pk);
-          }
-          if (!ok) {
-            failed = true;
-            break;
-          }
-          const float2 add = pg_two(pg_add2(sum[0], sum[1]));
-          l += add.x + add.y;
-          tc_wait_st();
           tc_fence_before();
-          mbar_arrive(b_p + 8 * (2 * s + h));
+          mbar_arrive(b_p + 16 * s + 8 * h);
         }
       }
       const size_t slot = size_t(int(blockIdx.x) + pc.unit) * 2 + t;
@@ -891,7 +945,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   if (*flag != 0 && tid == 0) atomicOr(A.status, 1);
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPgTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_held), "n"(kPgTmemCols) : "memory");
   }
 }
 

@@ -5,8 +5,8 @@ Bounds.  u = torch.finfo(t).eps / 2 is the largest relative rounding error of ty
 Rotation: fp32 sine and cosine are within 2^-22 of exact (their argument rounded to fp32 after
 an exact reduction, the functions' own 2 units, the scaling's rounding), products and sum
 add 2^-23 of |x1| + |x2|; then one rounding to t.  Attention: every probability is rounded to t
-once (u), scores carry the error of a D-term fp32 sum and of the exponential, and the output
-is rounded to t once."""
+once (u), scores carry the error of a D-term fp32 sum and of the exponential (2^-20), and the
+output is rounded to t once."""
 
 import torch
 
