@@ -99,11 +99,17 @@ struct PagedArgs {
 // time that memory takes for all of it (kOwnMem when every SM streams).
 template <int D>
 struct PgCost {
-  static constexpr int kPair = D == 128 ? 76 : 62;
+  static constexpr int kPair = D == 128 ? 70 : 58;
   static constexpr int kOne = D == 128 ? 38 : 32;
   static constexpr int kOwnMin = D == 128 ? 34 : 27;
   static constexpr int kOwnMem = D == 128 ? 43 : 28;
 };
+
+// a / b for b > 0, in 32 bits where they suffice (a 64-bit division takes several hundred clocks).
+__device__ __forceinline__ long long pg_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (long long)(unsigned(a) / unsigned(b));
+  return a / b;
+}
 
 struct PagedLine {
   int chunks;            // prefix chunks (0: nothing shared, or no sequence that has it all)
@@ -130,7 +136,7 @@ __device__ __forceinline__ PagedLine paged_line(const PagedArgs& A, int own_chun
   L.own_cost = imax(C::kOwnMin, C::kOwnMem - int(fminf(share, float(C::kOwnMem))));
   L.total = L.prefix_cost + own * L.own_cost;
   const int most = imax(own > 0 ? L.own_cost : 0, L.chunks == 0 ? 0 : L.pairs > 0 ? C::kPair : C::kOne);
-  L.per_cta = (L.total + A.ctas - 1) / A.ctas;
+  L.per_cta = pg_div(L.total + A.ctas - 1, A.ctas);
   if (L.per_cta < most) L.per_cta = most;
   return L;
 }
@@ -454,6 +460,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   grid_dependency_wait();  // lengths, table, query and cache rows are written
+  allow_dependents();      // the combine's CTAs take their places as this kernel's end
 
   // ---- the line: own chunks before each thread's run of sequences
   const int per = (A.batch + kPgThreads - 1) / kPgThreads;
@@ -511,10 +518,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   if (walk.lo < L.prefix_cost) {
     walk.own = false;
     walk.len = 0;
-    walk.h = int(walk.lo / L.head_cost);
+    walk.h = int(pg_div(walk.lo, L.head_cost));
     const long long r = walk.lo - walk.h * L.head_cost;
     const long long pair_cost = (long long)L.chunks * PgCost<D>::kPair;
-    walk.at = imin(int(r / pair_cost), L.groups - 1);  // the groups before the last are pairs
+    walk.at = imin(int(pg_div(r, pair_cost)), L.groups - 1);  // the groups before the last are pairs
     walk.unit = walk.h * L.groups + walk.at;
     walk.base = walk.h * L.head_cost + walk.at * pair_cost;
   } else {
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     if (walk.at < A.batch) {
       walk.len = paged_len(A, walk.at);
       const long long unit_cost = (long long)L.own_cost * paged_own_chunks(A, walk.len);
-      walk.h = int((walk.lo - walk.base) / unit_cost);
+      walk.h = int(pg_div(walk.lo - walk.base, unit_cost));
       walk.base += walk.h * unit_cost;
     }
     walk.unit = walk.at * A.heads_kv + walk.h;
@@ -559,8 +566,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     bool live = walk.next(A, L, pc), more = false;
     int page = live ? page_of(pc, pc.j0) : -1;
     for (; live && !failed; live = more, pc = ahead) {
-      more = walk.next(A, L, ahead);
-      const int first_page = more ? page_of(ahead, ahead.j0) : -1;  // in flight under this piece
       const bool narrow = pc.own || narrow_prefix;
       if (lane == 0) {
         int* bound = reinterpret_cast<int*>(A.bounds + (pc.own ? A.units : 0) + pc.unit);
@@ -595,6 +600,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | ((s_q + (narrow ? (slot - 2) * 1024 : slot * kTB)) >> 4) << 16;
         narrow ? ++thin : ++wide;
       }
+      more = walk.next(A, L, ahead);
+      const int first_page = more ? page_of(ahead, ahead.j0) : -1;  // in flight under this piece's chunks
       for (int j = pc.j0; j < pc.j1 && !failed; ++j) {
         const int next_page = j + 1 < pc.j1 ? page_of(pc, j + 1) : first_page;
         int at = page;
@@ -939,7 +946,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     }
   }
   if (failed) atomicOr(flag, 1);
-  allow_dependents();
   tc_fence_before();
   __syncthreads();
   if (*flag != 0 && tid == 0) atomicOr(A.status, 1);
@@ -965,68 +971,72 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
   const int b = int(blockIdx.x) / A.heads_kv, h = int(blockIdx.x) - b * A.heads_kv;
   grid_dependency_wait();
   allow_dependents();
+  // ---- where the partials are: CTAs [c.x, c.y] of the prefix unit and of the own unit (bounds are
+  // read beside the length, before it is known whether they count)
   const int len = paged_len(A, b);
-  // ---- where the partials are: CTAs [c0, c0 + np) of the prefix unit, [c1, c1 + no) of the own unit
-  int np = 0, no = 0, sub0 = 0, subs = 2;
-  size_t slot_p = 0, slot_o = 0, row_p = 0;
-  if (A.shared > 0 && len >= A.shared) {
-    const int tile = b / A.per_tile, grp = tile >> 1;
-    const bool pair = 2 * grp + 1 < A.tiles;
-    const int u = h * ((A.tiles + 1) / 2) + grp;
-    const int2 c = A.bounds[u];
-    np = c.y - c.x + 1;
-    slot_p = size_t(c.x + u) * 2;
-    sub0 = pair ? tile & 1 : 0;
-    subs = pair ? 1 : 2;
-    row_p = size_t(b - tile * A.per_tile) * G;
-  }
-  if (paged_own_chunks(A, len) > 0) {
-    const int u = b * A.heads_kv + h;
-    const int2 c = A.bounds[A.units + u];
-    no = c.y - c.x + 1;
-    slot_o = size_t(c.x + u) * 2;
-  }
-  const int n_p = np * subs, n = n_p + no * 2;
+  const int tile = b / A.per_tile, grp = tile >> 1, unit = b * A.heads_kv + h;
+  const int unit_p = h * ((A.tiles + 1) / 2) + grp;
+  const int2 cp = A.shared > 0 ? A.bounds[unit_p] : make_int2(0, -1), co = A.bounds[A.units + unit];
+  const bool has_p = A.shared > 0 && len >= A.shared, has_o = paged_own_chunks(A, len) > 0;
+  const bool pair = 2 * grp + 1 < A.tiles;
+  const int subs = pair ? 1 : 2, sub0 = pair ? tile & 1 : 0;  // streams of a prefix piece with this tile
+  const size_t slot_p = has_p ? size_t(cp.x + unit_p) * 2 : 0, slot_o = has_o ? size_t(co.x + unit) * 2 : 0;
+  const size_t row_p = size_t(b - tile * A.per_tile) * G;
+  const int n_p = has_p ? (cp.y - cp.x + 1) * subs : 0, n = n_p + (has_o ? (co.y - co.x + 1) * 2 : 0);
   auto part_p = [&](int i) { return slot_p + (subs == 2 ? i : 2 * i + sub0); };  // its [2]-slot
-  for (int g = warp; g < G; g += kPgCombineThreads / 32) {
-    float mx = kNegInf;
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = i < n_p ? A.ml_prefix[part_p(i) * kPgTile + row_p + g] : A.ml_own[(slot_o + i - n_p) * G + g];
-      mx = fmaxf(mx, ml.x);
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
-    float sum = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = i < n_p ? A.ml_prefix[part_p(i) * kPgTile + row_p + g] : A.ml_own[(slot_o + i - n_p) * G + g];
-      const float x = ml.x == kNegInf ? 0.f : pg_exp2(ml.x - mx);
-      if (ml.x != kNegInf) sum = fmaf(x, ml.y, sum);
-      w[g * n + i] = ml.x == kNegInf ? -1.f : x;  // -1: nothing there
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-    if (lane == 0) inv[g] = sum;
-  }
-  __syncthreads();
   constexpr int kWords = D / 4;
   const int items = G * kWords;                     // 16-byte words of the G rows, rows fastest
   const int teams = kPgCombineThreads / items;      // 1 to 16
   const int team = tid / items, item = tid - team * items;
   const int x = item / G, g = item - x * G;
+  auto word = [&](int i) {  // this thread's word of partial i
+    return *reinterpret_cast<const float4*>(
+        i < n_p ? A.o_prefix + (part_p(i) * kPgTile * kWords + size_t(x) * kPgTile + row_p + g) * 4
+                : A.o_own + ((slot_o + i - n_p) * G + g) * D + 4 * x);
+  };
+  constexpr int kAhead = 4;  // partials whose words are on their way while the weights are made
+  float4 v[kAhead];
+  if (team < teams) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (team + k * teams < n) v[k] = word(team + k * teams);
+  }
+  for (int gg = warp; gg < G; gg += kPgCombineThreads / 32) {
+    auto ml_of = [&](int i) {
+      return i < n_p ? A.ml_prefix[part_p(i) * kPgTile + row_p + gg] : A.ml_own[(slot_o + i - n_p) * G + gg];
+    };
+    const float2 first = lane < n ? ml_of(lane) : make_float2(kNegInf, 0.f);
+    float mx = first.x;
+    for (int i = lane + 32; i < n; i += 32) mx = fmaxf(mx, ml_of(i).x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
+    float sum = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float2 ml = i == lane ? first : ml_of(i);
+      const float f = ml.x == kNegInf ? 0.f : pg_exp2(ml.x - mx);
+      if (ml.x != kNegInf) sum = fmaf(f, ml.y, sum);
+      w[gg * n + i] = ml.x == kNegInf ? -1.f : f;  // -1: nothing there
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+    if (lane == 0) inv[gg] = sum;
+  }
+  __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (team < teams) {
-#pragma unroll 4
-    for (int i = team; i < n; i += teams) {
+    auto add = [&](int i, const float4& p) {
       const float f = w[g * n + i];
-      if (f < 0.f) continue;
-      const float* src = i < n_p ? A.o_prefix + (part_p(i) * kPgTile * kWords + size_t(x) * kPgTile + row_p + g) * 4
-                                 : A.o_own + ((slot_o + i - n_p) * G + g) * D + 4 * x;
-      const float4 v = *reinterpret_cast<const float4*>(src);
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
-    }
+      if (f < 0.f) return;
+      o.x = fmaf(f, p.x, o.x);
+      o.y = fmaf(f, p.y, o.y);
+      o.z = fmaf(f, p.z, o.z);
+      o.w = fmaf(f, p.w, o.w);
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (team + k * teams < n) add(team + k * teams, v[k]);
+#pragma unroll 4
+    for (int i = team + kAhead * teams; i < n; i += teams) add(i, word(i));
   }
   sums[tid] = o;
   __syncthreads();

@@ -53,6 +53,7 @@ class _AppendCall:
         if counts is not None and (counts.shape != (cache.batch,) or counts.dtype != torch.int32
                                    or counts.device != cache.device or not counts.is_contiguous()):
             raise ValueError(f"counts is a contiguous int32 [{cache.batch}] tensor on {cache.device}")
+        self.copies = any(self.copy)
         self.empty = not (tokens and cache.batch)
         k, v, q = (x if x is None else x.detach().contiguous() if c else x.detach()
                    for x, c in zip((k, v, q), self.copy))
@@ -157,7 +158,7 @@ class PagedKVCache:
         call = known.get(form)
         if call is None:
             call = known[form] = _AppendCall(self, k, v, q, counts)
-        if any(call.copy):
+        if call.copies:
             k, v, q = (x.contiguous() if c else x for x, c in zip((k, v, q), call.copy))
         q_out = None if q is None else torch.empty_like(q)
         if call.empty:
@@ -190,7 +191,7 @@ class PagedKVCache:
             call = known[form] = _AttendCall(self, q, shared_len, aligned)
         if call.copy:
             q = q.clone(memory_format=torch.contiguous_format)
-        out = torch.empty(call.shape, dtype=self.dtype, device=self._index)
+        out = q.new_empty(call.shape)
         if self.batch == 0:
             return out
         with _lib.on_device(self._index):

@@ -204,14 +204,19 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, inv_freq)
+        # neither is differentiable, so they need no saved-tensor hooks; their versions are
+        # compared in the backward pass, as torch does for saved tensors
+        ctx.kept = positions, inv_freq, positions._version, inv_freq._version
         ctx.how = interleaved, scale, inverse
         q_out, k_out = _launch(q, k, positions, inv_freq, interleaved, scale, inverse)
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
     def backward(ctx, dq, dk=None):
-        positions, inv_freq = ctx.saved_tensors
+        positions, inv_freq, *versions = ctx.kept
+        if versions != [positions._version, inv_freq._version]:
+            raise RuntimeError("the positions or frequencies of a rotary call were changed in place before its "
+                               "backward pass")
         interleaved, scale, inverse = ctx.how
         rest = (positions, inv_freq, interleaved, scale, not inverse)
         if not torch.is_grad_enabled():  # no graph of the backward pass is asked for

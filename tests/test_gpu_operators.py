@@ -141,6 +141,16 @@ def test_rotary_gradients_match_differences_and_reach_one_side_alone():
     torch.testing.assert_close(ddq, torch.full_like(q, 2.0), rtol=0, atol=2.0 ** -18)
 
 
+def test_rotary_refuses_a_backward_pass_at_changed_positions():
+    f = rope_frequencies(64)[0].to(DEV)
+    pos = torch.arange(3, device=DEV)
+    x = randn(gen(6), 1, 1, 3, 64, dtype=FP).requires_grad_(True)
+    y, _ = rotary(x, None, pos, f)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="changed in place"):
+        torch.autograd.grad(y.sum(), x)
+
+
 def test_rotary_in_a_graph_with_its_backward():
     """Forward and backward captured, after eager passes over the same leaf whose graphs are gone
     (torch ties a living graph's leaf to the stream it was made on, which no capture may join)."""
