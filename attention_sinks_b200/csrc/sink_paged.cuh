@@ -417,8 +417,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   static_assert(16 * kRing + 96 + 128 + 16 + 8 <= 464, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(g_bar + 464);
   int* flag = reinterpret_cast<int*>(g_bar + 468);
-  int* start = reinterpret_cast<int*>(g_bar + 472);               // first own sequence, chunks before it
-  int* scan = reinterpret_cast<int*>(g_bar + 480);                // [11] warp sums
+  int* scan = reinterpret_cast<int*>(g_bar + 472);                // [11] warp sums
+  int* start = reinterpret_cast<int*>(g_bar + 516);               // first own sequence, chunks before it, its length
   float2* g_ml = reinterpret_cast<float2*>(g_bar + 528);          // [2 streams][4 warps][8 rows] of narrow tiles
   uint32_t* steps = reinterpret_cast<uint32_t*>(g_bar + 528 + 2 * 4 * kPgNarrow * 8);  // [kPgSteps]
   static_assert(528 + 2 * 4 * kPgNarrow * 8 + 4 * kPgSteps <= G_::kBarBytes, "records");
@@ -500,10 +500,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     if (want >= own_unit * before && want < own_unit * (before + mine)) {
       int c = before;
       for (int b = b_lo; b < b_hi; ++b) {
-        const int n = paged_own_chunks(A, paged_len(A, b));
+        const int len = paged_len(A, b), n = paged_own_chunks(A, len);
         if (want < own_unit * (c + n)) {
           start[0] = b;
           start[1] = c;
+          start[2] = len;
           break;
         }
         c += n;
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     walk.len = -1;
     walk.h = 0;
     if (walk.at < A.batch) {
-      walk.len = paged_len(A, walk.at);
+      walk.len = start[2];
       const long long unit_cost = (long long)L.own_cost * paged_own_chunks(A, walk.len);
       walk.h = int(pg_div(walk.lo - walk.base, unit_cost));
       walk.base += walk.h * unit_cost;
@@ -585,17 +586,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           failed = true;
           break;
         }
-        if (lane == 0) {
-          const uint32_t bar = b_qfull + 8 * slot;
-          const uint32_t dst = s_q + (narrow ? (slot - 2) * 1024 : slot * kTB);
-          // a narrow tile's rows once for each warp of the warpgroup, 32 TMEM lanes apart
-          const int copies = narrow ? 4 : 1;
-          const CUtensorMap* map = pc.own ? &A.qgroup : &A.qtile;
-          const int seq = pc.own ? pc.which : (pc.which + t) * A.per_tile;
-          mbar_arrive_expect_tx(bar, (pc.own ? qrow_bytes : qrow_bytes * A.per_tile) * copies);
-          for (int x = 0; x < kBoxes; ++x)
-            for (int c = 0; c < copies; ++c)
-              tma_load_3d(dst + x * kBox + c * 32 * 128, map, 64 * x, pc.h * A.group, seq, bar);
+        // a narrow tile's rows once for each warp of the warpgroup, 32 TMEM lanes apart
+        const int copies = narrow ? 4 : 1;
+        const uint32_t bar = b_qfull + 8 * slot;
+        if (lane == 0) mbar_arrive_expect_tx(bar, (pc.own ? qrow_bytes : qrow_bytes * A.per_tile) * copies);
+        __syncwarp();
+        if (lane < copies * kBoxes) {  // a lane per copy
+          const int x = lane / copies, c = lane - x * copies;
+          tma_load_3d(s_q + (narrow ? (slot - 2) * 1024 : slot * kTB) + x * kBox + c * 32 * 128,
+                      pc.own ? &A.qgroup : &A.qtile, 64 * x, pc.h * A.group,
+                      pc.own ? pc.which : (pc.which + t) * A.per_tile, bar);
         }
         q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | ((s_q + (narrow ? (slot - 2) * 1024 : slot * kTB)) >> 4) << 16;
         narrow ? ++thin : ++wide;
