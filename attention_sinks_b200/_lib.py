@@ -521,15 +521,25 @@ def form_of(x: torch.Tensor | None):
 
 
 class RowsArg:
-    """A sink_rows_t argument that is described once and pointed at a tensor per call."""
+    """A sink_rows_t argument, described once (from any tensor of its form, a meta one too) and
+    pointed at a tensor per call."""
 
     def __init__(self, t: torch.Tensor):
-        self.rows = rows_desc(t)
+        if t.dim() != 4 or t.stride(-1) != 1:
+            raise ValueError(f"expected a [B, H, n, D] tensor with unit last stride, got {tuple(t.shape)} "
+                             f"strides {t.stride()}")
+        self.rows = Rows(0, dtype_code(t.dtype), t.shape[1], t.shape[2], 0, t.stride(0), t.stride(1), t.stride(2))
         self.ref = ctypes.byref(self.rows)
 
     def at(self, t: torch.Tensor):
         self.rows.data = t.data_ptr()
         return self.ref
+
+
+def layout_of(t: torch.Tensor, copied: bool) -> torch.Tensor:
+    """A meta tensor in the layout of `t`, or of its contiguous copy."""
+    like = torch.empty(t.shape, dtype=t.dtype, device="meta")
+    return like if copied else like.as_strided(t.shape, t.stride())
 
 
 def raw_stream(index: int) -> int:

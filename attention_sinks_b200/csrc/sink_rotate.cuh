@@ -43,7 +43,7 @@ struct RotArgs {
   // dense positions: pos[b * pos_sb + t]
   const int64_t* pos;
   int64_t pos_sb;
-  // paged: token t of sequence b has position lens[b] - counts[b] + t (t < counts[b] <= tokens)
+  // paged: token t < counts[b] (at most `tokens`) of sequence b has position lens[b] - counts[b] + t
   const int32_t* lens;
   const int32_t* counts;   // null: `tokens` for every sequence
   const int32_t* table;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm) sink_rotate_kernel
   if (token >= unsigned(A.batch) * unsigned(A.tokens)) return;
   const int b = int(token / unsigned(A.tokens)), t = int(token - unsigned(b) * unsigned(A.tokens));
   int count = A.tokens;
-  if (A.counts != nullptr) count = A.counts[b];
+  if (A.counts != nullptr) count = imax(0, imin(A.counts[b], A.tokens));
   const int rows = A.seg[0].heads + A.seg[1].heads + A.seg[2].heads;  // unused segments have none
 
   auto segment_of = [&](int r, int& h) {

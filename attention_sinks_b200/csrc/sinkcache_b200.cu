@@ -1064,10 +1064,10 @@ const char* sink_strerror(int32_t code) {
   switch (code) {
     case SINK_OK: return "ok";
     case SINK_EINVAL: return "sinkcache_b200: size or index out of range";
-    case SINK_EDTYPE: return "sinkcache_b200: unsupported dtype combination (K fp32 or model dtype; V, q, new rows in the model dtype bf16/fp16/fp32)";
-    case SINK_EHEADDIM: return "sinkcache_b200: head_dim must be 64, 128 or 256";
+    case SINK_EDTYPE: return "sinkcache_b200: unsupported dtype combination (K fp32 or model dtype; V, q, new rows in the model dtype bf16/fp16/fp32; paged attention in bf16/fp16; one dtype per rotation or paged call)";
+    case SINK_EHEADDIM: return "sinkcache_b200: head_dim must be 64, 128 or 256 (paged attention: 64 or 128; rotation and paged append: up to 512)";
     case SINK_EGROUP: return "sinkcache_b200: heads_q / heads_kv must be an integer between 1 and 8";
-    case SINK_ELAYOUT: return "sinkcache_b200: cache rows must be contiguous and 16-byte aligned";
+    case SINK_ELAYOUT: return "sinkcache_b200: cache rows must be contiguous and 16-byte aligned (paged attention: pages, heads and queries too)";
     case SINK_EWORKSPACE: return "sinkcache_b200: workspace missing or smaller than sink_workspace_bytes()";
     case SINK_EDEVICE: return "sinkcache_b200: no usable CUDA device";
     case SINK_ESCRATCH: return "sinkcache_b200: request needs more than the 16 MiB static scratch of sink_decode_attention_noalloc; use sink_decode_attention with a workspace";

@@ -25,18 +25,17 @@ import torch
 from . import _lib
 from .rope import device_frequencies, rotation
 
-# Scratch of `attend`, one buffer per (device, stream): calls on one stream run in order, so they
-# can share one.  Inside a graph capture a fresh one comes from the graph's own pool, so that
-# two graphs never share.
-_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
-
-
 def _scratch(nbytes: int, index: int, stream: int) -> torch.Tensor:
+    """Scratch of `attend`, one buffer per (thread, device, stream): a call's two launches follow
+    each other on their stream, so one thread's calls there can share one; another thread's
+    launches may come between.  Inside a graph capture a fresh one comes from the graph's own
+    pool, so that two graphs never share."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=index)
-    buf = _SCRATCH.get((index, stream))
+    buffers = _lib.forms("scratch")
+    buf = buffers.get((index, stream))
     if buf is None or buf.numel() < nbytes:
-        buf = _SCRATCH[index, stream] = torch.empty(nbytes, dtype=torch.uint8, device=index)
+        buf = buffers[index, stream] = torch.empty(nbytes, dtype=torch.uint8, device=index)
     return buf
 
 
@@ -55,8 +54,7 @@ class _AppendCall:
             raise ValueError(f"counts is a contiguous int32 [{cache.batch}] tensor on {cache.device}")
         self.copies = any(self.copy)
         self.empty = not (tokens and cache.batch)
-        k, v, q = (x if x is None else x.detach().contiguous() if c else x.detach()
-                   for x, c in zip((k, v, q), self.copy))
+        k, v, q = (x if x is None else _lib.layout_of(x, c) for x, c in zip((k, v, q), self.copy))
         self.k, self.v = _lib.RowsArg(k), _lib.RowsArg(v)
         if q is not None:
             self.q, self.q_out = _lib.RowsArg(q), _lib.RowsArg(torch.empty_like(q))
@@ -72,7 +70,7 @@ class _AttendCall:
         self.copy = (not aligned or q.stride(-1) != 1 or q.stride(0) % 8 or q.stride(1) % 8
                      or min(q.stride(0), q.stride(1)) < d)
         self.shape = (b, 1, hq, d)
-        self.q = _lib.RowsArg(q.detach().clone(memory_format=torch.contiguous_format) if self.copy else q.detach())
+        self.q = _lib.RowsArg(_lib.layout_of(q, self.copy))
         # shapes that the kernel refuses need nothing: the call says why
         self.workspace = max(256, _lib.paged_workspace_bytes(b, cache.heads_kv, hq, d, shared_len,
                                                              _lib.sm_count(cache.device)))
@@ -151,7 +149,8 @@ class PagedKVCache:
         rows of sequence b: rows lens[b] - counts[b] .. lens[b] - 1, k rotated to those
         positions.  Returns q [B, Hq, T, D] rotated to them too, in one launch (None without q).
         Tokens from counts[b] on, and all of an idle sequence's (lens 0), are not stored; their
-        q rows come back as zeros.  counts: int32 [B] on the device."""
+        q rows come back as zeros.  counts: int32 [B] on the device.  Sequences may share pages that
+        they read; of two that append to one slot, one row stays."""
         self._no_gradients(k, v, q)
         form = (self._like, _lib.form_of(k), _lib.form_of(v), _lib.form_of(q), _lib.form_of(counts))
         known = _lib.forms("append")

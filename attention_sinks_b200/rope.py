@@ -142,8 +142,9 @@ class _RotaryCall:
             raise ValueError(f"positions are whole numbers on {device}, got {positions.dtype} on {positions.device}")
         if positions.shape not in ((t,), (b, t), (1, t)):
             raise ValueError(f"positions are [{t}] or [{b}, {t}], got {tuple(positions.shape)}")
-        if 2 * inv_freq.numel() > d or d > 512:
-            raise ValueError(f"{2 * inv_freq.numel()} rotated dims of a head of {d} (at most 512)")
+        if inv_freq.dim() != 1 or 2 * inv_freq.numel() > d or d > 512:
+            raise ValueError(f"inv_freq {tuple(inv_freq.shape)} is not one-dimensional, or rotates more than a head of "
+                             f"{d} dims (at most 512)")
         self.device, self.index = device, device.index
         self.batch, self.dim = b, d
         # what a call has to convert first
@@ -152,11 +153,11 @@ class _RotaryCall:
         self.copy_positions = positions.dtype != torch.int64 or (t > 1 and positions.stride(-1) != 1)
         self.copy_freq = inv_freq.dtype != torch.float64 or inv_freq.device != device or not inv_freq.is_contiguous()
         self.empty = not (q.numel() or (k is not None and k.numel()))
-        q = q.detach().contiguous() if self.copy_q else q.detach()
-        self.q, self.q_out = _lib.RowsArg(q), _lib.RowsArg(torch.empty_like(q))
+        like = _lib.layout_of(q, self.copy_q)
+        self.q, self.q_out = _lib.RowsArg(like), _lib.RowsArg(torch.empty_like(like))
         if k is not None:
-            k = k.detach().contiguous() if self.copy_k else k.detach()
-            self.k, self.k_out = _lib.RowsArg(k), _lib.RowsArg(torch.empty_like(k))
+            like = _lib.layout_of(k, self.copy_k)
+            self.k, self.k_out = _lib.RowsArg(like), _lib.RowsArg(torch.empty_like(like))
         several = positions.dim() == 2 and positions.shape[0] > 1
         self.pos_stride = 0 if not several else t if self.copy_positions else positions.stride(0)
         self.rot = _lib.Rotation(0, inv_freq.numel(), 0, 1.0, 0)

@@ -425,8 +425,8 @@ typedef struct sink_paged_kv {
 /*
  * Append: the first counts[b] tokens of k_new / v_new [batch, heads_kv, n, head_dim] become rows
  * lens[b] - counts[b] .. lens[b] - 1 of sequence b, k rotated to its position on the way (rot
- * NULL: as it is).  counts: device int32 [batch], NULL for n everywhere.  Tokens from counts[b]
- * on, and tokens whose position is negative (an idle sequence: lens 0), are not written.
+ * NULL: as it is).  counts: device int32 [batch] (more than n counts as n), NULL for n
+ * everywhere.  Tokens from counts[b] on, and tokens whose position is negative (an idle sequence: lens 0), are not written.
  * q / q_out (both or neither; [batch, heads, n, head_dim]): rotated to the same positions in the
  * same launch, zeros for tokens that are not written.  Two sequences that append to one slot
  * leave one of the two rows there.

@@ -83,6 +83,39 @@ def test_rotary_takes_any_strides(layout):
         ref.assert_bounded(y, want, ref.rotate_bound(x, want, f, False, 1.0, BF))
 
 
+@pytest.mark.parametrize("positions", ["int32", "strided", "one row", "column"])
+def test_rotary_takes_any_positions(positions):
+    g, f = gen(4), rope_frequencies(64)[0]
+    q = randn(g, 2, 3, 10, 64)
+    pos = torch.randint(0, 9999, (2, 10), generator=g, device=DEV)
+    if positions == "int32":
+        given = pos.to(torch.int32)
+    elif positions == "strided":
+        given = torch.stack((pos, pos + 1), -1).flatten(1)[:, ::2]
+    elif positions == "one row":
+        given, pos = pos[:1], pos[:1].expand(2, 10)
+    else:
+        given = pos.t().contiguous().t()
+    y, _ = rotary(q, None, given, f)  # frequencies from the host are copied per call
+    want = ref.rotate(q, pos, f)
+    ref.assert_bounded(y, want, ref.rotate_bound(q, want, f, False, 1.0, BF))
+
+
+def test_rotary_refusals():
+    f = rope_frequencies(64)[0].to(DEV)
+    q, pos = torch.zeros(2, 3, 5, 64, device=DEV), torch.arange(5, device=DEV)
+    for bad in (lambda: rotary(q[0], None, pos, f), lambda: rotary(q, q[:1], pos, f),
+                lambda: rotary(q, q.half(), pos, f), lambda: rotary(q, q[:, :, :4], pos, f),
+                lambda: rotary(q, None, pos[:4], f), lambda: rotary(q, None, pos.float(), f),
+                lambda: rotary(q, None, pos.cpu(), f), lambda: rotary(q, None, pos, torch.cat((f, f))),
+                lambda: rotary(q, None, pos, f.view(2, 16)),
+                lambda: rotary(torch.zeros(1, 1, 5, 1024, device=DEV), None, pos, f)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        rotary(q.double(), None, pos, f)
+
+
 def test_rotary_empty_and_infinite():
     f = rope_frequencies(64)[0].to(DEV)
     q, k = rotary(torch.empty(2, 4, 0, 64, device=DEV), torch.empty(2, 1, 0, 64, device=DEV),
@@ -331,6 +364,98 @@ def test_paged_attention_strides_and_layouts():
     sub = PagedKVCache(cache.k_pages, cache.v_pages, table[:, 5:5 + cache.block_table.shape[1]], cache.lens)
     q = randn(g, 3, 4, 1, 128)
     assert torch.equal(sub.attend(q), cache.attend(q))
+
+
+@pytest.mark.parametrize("shared", [0, 32])
+def test_paged_attention_many_sequences(shared):
+    """More sequences than the kernel has threads, idle ones among them."""
+    g = gen(20 + shared)
+    lens = [0 if i % 7 == 3 else shared + (i * 13) % 40 + 1 for i in range(1100)]
+    cache = make_cache(g, lens, 1, 16, 64, shared=shared)
+    check_attend(cache, randn(g, 1100, 2, 1, 64), shared)
+
+
+def test_paged_attention_refusals():
+    g = gen(27)
+    cache = make_cache(g, [40, 20], 2, 16, 64)
+    q, k = randn(g, 2, 4, 1, 64), randn(g, 2, 2, 1, 64)
+    for bad in (lambda: cache.attend(q[:1]), lambda: cache.attend(q.half()), lambda: cache.attend(randn(g, 2, 4, 2, 64)),
+                lambda: cache.attend(q.cpu()), lambda: cache.append(k, k[:1]), lambda: cache.append(q, k),
+                lambda: cache.append(k, k, counts=torch.zeros(2, device=DEV)),
+                lambda: cache.append(k, k, counts=torch.zeros(3, dtype=torch.int32, device=DEV)),
+                lambda: cache.append(k, k, q=randn(g, 2, 4, 3, 64)),
+                lambda: PagedKVCache(cache.k_pages, cache.v_pages[:1], cache.block_table, cache.lens),
+                lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.block_table.long(), cache.lens),
+                lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.block_table, cache.lens[:1]),
+                lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.block_table, cache.lens.cpu()),
+                lambda: PagedKVCache(cache.k_pages.transpose(2, 3), cache.v_pages.transpose(2, 3), cache.block_table,
+                                     cache.lens),
+                lambda: PagedKVCache(cache.k_pages, cache.v_pages, cache.block_table, cache.lens,
+                                     inv_freq=torch.ones(33, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: cache.attend(q, shared_len=8), lambda: cache.attend(q, shared_len=-16),
+                lambda: cache.attend(q, shared_len=1 << 20), lambda: cache.attend(randn(g, 2, 3, 1, 64)),
+                lambda: cache.attend(randn(g, 2, 18, 1, 64)), lambda: cache.attend(q, scale=float("nan")),
+                lambda: make_cache(g, [4], 1, 16, 64, FP).attend(randn(g, 1, 1, 1, 64, dtype=FP)),
+                lambda: make_cache(g, [4], 1, 16, 80).attend(randn(g, 1, 1, 1, 80)),
+                lambda: make_cache(g, [4], 1, 48, 64).attend(randn(g, 1, 1, 1, 64))):
+        with pytest.raises(RuntimeError, match="sinkcache_b200"):
+            bad()
+    with pytest.raises(RuntimeError, match="gradients"):
+        cache.attend(q.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="gradients"):
+        cache.append(k.clone().requires_grad_(True), k)
+    with torch.no_grad():
+        cache.attend(q.clone().requires_grad_(True))
+    cache.check_status()
+
+
+def test_paged_calls_on_nothing():
+    pools = torch.zeros(3, 2, 16, 64, device=DEV, dtype=BF)
+    none = PagedKVCache(pools, pools.clone(), torch.zeros(0, 4, dtype=torch.int32, device=DEV),
+                        torch.zeros(0, dtype=torch.int32, device=DEV))
+    assert none.attend(torch.zeros(0, 4, 1, 64, device=DEV, dtype=BF)).shape == (0, 1, 4, 64)
+    some = make_cache(gen(26), [40, 20], 2, 16, 64)
+    before = some.k_pages.clone()
+    q = some.append(*(torch.zeros(2, 2, 0, 64, device=DEV, dtype=BF) for _ in range(2)),
+                    q=torch.zeros(2, 4, 0, 64, device=DEV, dtype=BF))
+    assert q.shape == (2, 4, 0, 64) and torch.equal(some.k_pages.view(torch.int16), before.view(torch.int16))
+
+
+def test_append_of_more_than_there_is():
+    """Counts past the tokens given are those tokens, lengths below zero nothing."""
+    g = gen(28)
+    cache = make_cache(g, [40, 20, 20], 2, 16, 64, fill=0.0)
+    k, v = randn(g, 3, 2, 4, 64), randn(g, 3, 2, 4, 64)
+    cache.lens[2] = -3
+    kept = ref.gather(cache.v_pages, cache.block_table[2], 20)
+    cache.append(k, v, counts=torch.tensor([9, -2, 4], dtype=torch.int32, device=DEV))
+    cache.check_status()
+    assert torch.equal(ref.gather(cache.v_pages, cache.block_table[0], 40)[:, 36:], v[0].double())
+    assert torch.equal(ref.gather(cache.v_pages, cache.block_table[2], 20), kept)
+    assert not cache.attend(randn(g, 3, 4, 1, 64))[2].any()
+
+
+def test_attend_from_two_threads_on_one_stream():
+    import threading
+    g = gen(29)
+    caches = [make_cache(g, [1500 + 31 * i for i in range(16)], 8, 64, 128, shared=1024) for _ in range(2)]
+    qs = [randn(g, 16, 16, 1, 128) for _ in range(2)]
+    want = [c.attend(q, shared_len=1024) for c, q in zip(caches, qs)]
+    wrong = []
+
+    def work(i):
+        for _ in range(200):
+            if not torch.equal(caches[i].attend(qs[i], shared_len=1024), want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_paged_attention_repeats_bit_for_bit():
