@@ -460,7 +460,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   grid_dependency_wait();  // lengths, table, query and cache rows are written
-  allow_dependents();      // the combine's CTAs take their places as this kernel's end
 
   // ---- the line: own chunks before each thread's run of sequences
   const int per = (A.batch + kPgThreads - 1) / kPgThreads;
@@ -659,7 +658,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     // are then the same in every lane for the compiler too, and stay in uniform registers (issued
     // from inside a one-lane branch an MMA took 57 clocks, 30 this way).
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | (A.negate ? kPgNegateA : 0u);
+    const uint32_t negate = A.negate ? kPgNegateA : 0u;
+    const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | negate, idesc_whole = pg_idesc(kFmt, kPgKeys, false) | negate;
     const uint64_t desc = tc_desc(0, 16);
     const bool leader = pg_elect();
     int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest K
@@ -685,6 +685,27 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         if (failed) break;
       }
       const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
+      if (many == 1) {
+        // One step on the chunk: its 128 keys in one go (an MMA of 64 keys holds the tensor core as
+        // long as one of 128).
+        const int s = n & 1;
+        if (n >= 2 && (!pg_warp_wait(b_pv + 16 * s, ((n >> 1) - 1) & 1) ||
+                       !pg_warp_wait(b_pv + 16 * s + 8, ((n >> 1) - 1) & 1))) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t qd = desc + (rec >> 16);
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
+            tc_mma(s * 128, qd + off, kd + off, idesc_whole, kk > 0);
+          }
+          tc_commit(b_s + 16 * s);
+          tc_commit(b_s + 16 * s + 8);
+        }
+      } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll 1
@@ -707,6 +728,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           }
         }
         if (failed) break;
+      }
       }
       if (failed) break;
       if (leader) {
@@ -946,6 +968,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     }
   }
   if (failed) atomicOr(flag, 1);
+  allow_dependents();  // (at the start, the waiting combine made 2 streams on a 1K prompt 1 us slower)
   tc_fence_before();
   __syncthreads();
   if (*flag != 0 && tid == 0) atomicOr(A.status, 1);
