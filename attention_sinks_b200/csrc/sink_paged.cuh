@@ -96,13 +96,17 @@ struct PagedArgs {
 
 // Costs of a chunk in units of 64 clocks of one SM, by measurement: one tile or a pair of tiles on
 // it, and an own chunk, at least kOwnMin and, where memory bounds the own work, its share of the
-// time that memory takes for all of it (kOwnMem when every SM streams).
+// time that memory takes for all of it (kOwnMem when every SM streams); kUnit for each own unit,
+// its query and the join of its result.  (Without kUnit the CTAs of one-chunk units finish last: 64
+// sequences with 4K shared and 32 own rows 44.5 us without, 43.2 with 14, 44.4 with 30, 45.5 with
+// 40; 64 sequences of 512 own rows, units all alike, 46.0 without and 46.7 with 14.)
 template <int D>
 struct PgCost {
   static constexpr int kPair = D == 128 ? 70 : 58;
   static constexpr int kOne = D == 128 ? 38 : 32;
   static constexpr int kOwnMin = D == 128 ? 34 : 27;
   static constexpr int kOwnMem = D == 128 ? 43 : 28;
+  static constexpr int kUnit = 14;
 };
 
 // a / b for b > 0, in 32 bits where they suffice (a 64-bit division takes several hundred clocks).
@@ -122,7 +126,7 @@ struct PagedLine {
 };
 
 template <int D>
-__device__ __forceinline__ PagedLine paged_line(const PagedArgs& A, int own_chunks, bool prefix) {
+__device__ __forceinline__ PagedLine paged_line(const PagedArgs& A, int own_chunks, int own_seqs, bool prefix) {
   using C = PgCost<D>;
   PagedLine L;
   L.chunks = prefix ? (A.shared + kPgKeys - 1) / kPgKeys : 0;
@@ -134,8 +138,8 @@ __device__ __forceinline__ PagedLine paged_line(const PagedArgs& A, int own_chun
   const long long own = (long long)own_chunks * A.heads_kv;
   const float share = own > 0 ? float(L.prefix_cost) / float(own) : 0.f;
   L.own_cost = imax(C::kOwnMin, C::kOwnMem - int(fminf(share, float(C::kOwnMem))));
-  L.total = L.prefix_cost + own * L.own_cost;
-  const int most = imax(own > 0 ? L.own_cost : 0, L.chunks == 0 ? 0 : L.pairs > 0 ? C::kPair : C::kOne);
+  L.total = L.prefix_cost + own * L.own_cost + (long long)own_seqs * A.heads_kv * C::kUnit;
+  const int most = imax(own > 0 ? C::kUnit + L.own_cost : 0, L.chunks == 0 ? 0 : L.pairs > 0 ? C::kPair : C::kOne);
   L.per_cta = pg_div(L.total + A.ctas - 1, A.ctas);
   if (L.per_cta < most) L.per_cta = most;
   return L;
@@ -151,13 +155,18 @@ __device__ __forceinline__ int paged_own_chunks(const PagedArgs& A, int len) {
   return (len - paged_own_row(A, len) + kPgKeys - 1) / kPgKeys;
 }
 
-// Chunks [j0, j1) of the unit at `base`, n chunks of cost w (n * w < 2^32), that start in [lo, hi).
-__device__ __forceinline__ void paged_span(long long lo, long long hi, long long base, int n, int w, int& j0, int& j1) {
-  const unsigned all = unsigned(n) * unsigned(w);
-  const unsigned a = lo <= base ? 0u : lo - base >= all ? all : unsigned(lo - base);
-  const unsigned e = hi - base >= all ? all : unsigned(hi - base);  // hi > base
-  j0 = int((a + w - 1) / w);
-  j1 = int((e + w - 1) / w);
+// Chunks [j0, j1) of the unit at `base`, n chunks of cost w after a cost u (u + n * w < 2^32), that
+// start in [lo, hi).  The first starts at the base, the others behind u and those before them.
+__device__ __forceinline__ void paged_span(long long lo, long long hi, long long base, int n, int w, int u, int& j0,
+                                           int& j1) {
+  auto started = [&](long long x) -> int {  // chunks that start before x
+    if (x <= base) return 0;
+    const long long d = x - base;
+    if (d >= (long long)u + (long long)n * w) return n;
+    return d <= u + w ? 1 : int((unsigned(d) - unsigned(u) + unsigned(w) - 1) / unsigned(w));
+  };
+  j0 = started(lo);
+  j1 = started(hi);
 }
 
 struct PagedPiece {
@@ -178,7 +187,7 @@ struct PagedWalk {
 
   __device__ __forceinline__ bool next(const PagedArgs& A, const PagedLine& L, PagedPiece& p) {
     while (base < hi) {
-      int n, w;
+      int n, w, u = 0;
       if (!own) {
         if (unit >= L.units) {
           own = true;
@@ -196,6 +205,7 @@ struct PagedWalk {
         if (len < 0) len = paged_len(A, at);
         n = paged_own_chunks(A, len);
         w = L.own_cost;
+        u = unit_cost;
         p.which = at;
         p.pair = false;
       }
@@ -211,8 +221,8 @@ struct PagedWalk {
         len = -1;
         continue;
       }
-      paged_span(lo, hi, base, n, w, p.j0, p.j1);
-      base += (long long)n * w;
+      paged_span(lo, hi, base, n, w, u, p.j0, p.j1);
+      base += u + (long long)n * w;
       ++unit;
       if (own) {
         if (++h == A.heads_kv) {
@@ -228,7 +238,7 @@ struct PagedWalk {
     }
     return false;
   }
-  int cost_pair, cost_one;
+  int cost_pair, cost_one, unit_cost;
 };
 
 // ------------------------------------------------------------------ helpers
@@ -412,16 +422,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   const uint32_t s_q = base, s_ring = base + 2 * kTB, s_bar = s_ring + kRing * kTB;
   // mbarriers: full, empty [kRing]; qfull, qempty [6]; s, p, pv [stream * 2 + half]; rec [4]; wg [stream]; done
   const uint32_t b_full = s_bar, b_empty = b_full + 8 * kRing, b_qfull = b_empty + 8 * kRing, b_qempty = b_qfull + 48;
-  const uint32_t b_s = b_qempty + 48, b_p = b_s + 32, b_pv = b_p + 32, b_rec = b_pv + 32, b_wg = b_rec + 32, b_done = b_wg + 16;
+  const uint32_t b_s = b_qempty + 48, b_p = b_s + 32, b_pv = b_p + 32, b_rec = b_pv + 32;
+  const uint32_t b_wg = b_rec + 32, b_done = b_wg + 16;
   unsigned char* g_bar = gbase + (s_bar - base);
   static_assert(16 * kRing + 96 + 128 + 16 + 8 <= 464, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(g_bar + 464);
   int* flag = reinterpret_cast<int*>(g_bar + 468);
-  int* scan = reinterpret_cast<int*>(g_bar + 472);                // [11] warp sums
-  int* start = reinterpret_cast<int*>(g_bar + 516);               // first own sequence, chunks before it, its length
-  float2* g_ml = reinterpret_cast<float2*>(g_bar + 528);          // [2 streams][4 warps][8 rows] of narrow tiles
-  uint32_t* steps = reinterpret_cast<uint32_t*>(g_bar + 528 + 2 * 4 * kPgNarrow * 8);  // [kPgSteps]
-  static_assert(528 + 2 * 4 * kPgNarrow * 8 + 4 * kPgSteps <= G_::kBarBytes, "records");
+  int* start = reinterpret_cast<int*>(g_bar + 472);             // first own sequence, its length, cost before (64-bit)
+  long long* scan = reinterpret_cast<long long*>(g_bar + 488);  // [11] warp sums
+  float2* g_ml = reinterpret_cast<float2*>(g_bar + 576);        // [2 streams][4 warps][8 rows] of narrow tiles
+  uint32_t* steps = reinterpret_cast<uint32_t*>(g_bar + 576 + 2 * 4 * kPgNarrow * 8);  // [kPgSteps]
+  static_assert(576 + 2 * 4 * kPgNarrow * 8 + 4 * kPgSteps <= G_::kBarBytes, "records");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -443,7 +454,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     mbar_init(b_done, 2);
     *flag = 0;
     start[0] = A.batch;
-    start[1] = 0;
+    start[1] = start[2] = start[3] = 0;
     fence_mbar_init();
   }
   if (tid == 32 * kPgLoadWarp) {
@@ -464,49 +475,54 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   // ---- the line: own chunks before each thread's run of sequences
   const int per = (A.batch + kPgThreads - 1) / kPgThreads;
   const int b_lo = imin(tid * per, A.batch), b_hi = imin(b_lo + per, A.batch);
-  int mine = 0;
+  long long mine = 0;  // chunks, and in the upper half sequences that have any
   bool full = false;
   for (int b = b_lo; b < b_hi; ++b) {
-    const int n = paged_len(A, b);
-    mine += paged_own_chunks(A, n);
-    full |= n >= A.shared;
+    const int len = paged_len(A, b), n = paged_own_chunks(A, len);
+    mine += n > 0 ? (1ll << 32) + n : 0;
+    full |= len >= A.shared;
     if (blockIdx.x == 0 && A.lens[b] > A.table_width * A.page_size) atomicOr(A.status, 2);
   }
-  int before = mine;
+  long long before = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int x = __shfl_up_sync(kFull, before, off);
+    const long long x = __shfl_up_sync(kFull, before, off);
     if (lane >= off) before += x;
   }
   if (lane == 31) scan[warp] = before;
   const bool prefix = __syncthreads_or(full) != 0 && A.shared > 0;
-  int own_chunks = 0;
+  long long all = 0;
 #pragma unroll
   for (int w = 0; w < kPgThreads / 32; ++w) {
     if (w < warp) before += scan[w];
-    own_chunks += scan[w];
+    all += scan[w];
   }
   before -= mine;
-  const PagedLine L = paged_line<D>(A, own_chunks, prefix);
+  const PagedLine L = paged_line<D>(A, int(all), int(all >> 32), prefix);
   PagedWalk walk;
   walk.lo = L.per_cta * blockIdx.x;
   walk.hi = walk.lo + L.per_cta < L.total ? walk.lo + L.per_cta : L.total;
   walk.cost_pair = PgCost<D>::kPair;
   walk.cost_one = PgCost<D>::kOne;
-  const long long own_unit = (long long)L.own_cost * A.heads_kv;
+  walk.unit_cost = PgCost<D>::kUnit;
+  // cost of the own work of `n` (chunks, sequences) of all heads
+  auto own_cost = [&](long long n) {
+    return ((n & 0xffffffffll) * L.own_cost + (n >> 32) * PgCost<D>::kUnit) * A.heads_kv;
+  };
   if (mine > 0) {  // the sequence whose work holds position lo
     const long long want = walk.lo - L.prefix_cost;
-    if (want >= own_unit * before && want < own_unit * (before + mine)) {
-      int c = before;
+    if (want >= own_cost(before) && want < own_cost(before + mine)) {
+      long long c = before;
       for (int b = b_lo; b < b_hi; ++b) {
         const int len = paged_len(A, b), n = paged_own_chunks(A, len);
-        if (want < own_unit * (c + n)) {
+        const long long next = c + (n > 0 ? (1ll << 32) + n : 0);
+        if (want < own_cost(next)) {
           start[0] = b;
-          start[1] = c;
-          start[2] = len;
+          start[1] = len;
+          *reinterpret_cast<long long*>(start + 2) = own_cost(c);
           break;
         }
-        c += n;
+        c = next;
       }
     }
   }
@@ -527,12 +543,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   } else {
     walk.own = true;
     walk.at = start[0];
-    walk.base = L.prefix_cost + own_unit * start[1];
+    walk.base = L.prefix_cost + *reinterpret_cast<const long long*>(start + 2);
     walk.len = -1;
     walk.h = 0;
     if (walk.at < A.batch) {
-      walk.len = start[2];
-      const long long unit_cost = (long long)L.own_cost * paged_own_chunks(A, walk.len);
+      walk.len = start[1];
+      const long long unit_cost = (long long)L.own_cost * paged_own_chunks(A, walk.len) + PgCost<D>::kUnit;
       walk.h = int(pg_div(walk.lo - walk.base, unit_cost));
       walk.base += walk.h * unit_cost;
     }
@@ -587,16 +603,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         }
         // a narrow tile's rows once for each warp of the warpgroup, 32 TMEM lanes apart
         const int copies = narrow ? 4 : 1;
-        const uint32_t bar = b_qfull + 8 * slot;
+        const uint32_t bar = b_qfull + 8 * slot, dst = s_q + (narrow ? (slot - 2) * 1024 : slot * kTB);
         if (lane == 0) mbar_arrive_expect_tx(bar, (pc.own ? qrow_bytes : qrow_bytes * A.per_tile) * copies);
         __syncwarp();
         if (lane < copies * kBoxes) {  // a lane per copy
           const int x = lane / copies, c = lane - x * copies;
-          tma_load_3d(s_q + (narrow ? (slot - 2) * 1024 : slot * kTB) + x * kBox + c * 32 * 128,
+          tma_load_3d(dst + x * kBox + c * 32 * 128,
                       pc.own ? &A.qgroup : &A.qtile, 64 * x, pc.h * A.group,
                       pc.own ? pc.which : (pc.which + t) * A.per_tile, bar);
         }
-        q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | ((s_q + (narrow ? (slot - 2) * 1024 : slot * kTB)) >> 4) << 16;
+        q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | (dst >> 4) << 16;
         narrow ? ++thin : ++wide;
       }
       more = walk.next(A, L, ahead);
@@ -659,7 +675,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     // from inside a one-lane branch an MMA took 57 clocks, 30 this way).
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t negate = A.negate ? kPgNegateA : 0u;
-    const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | negate, idesc_whole = pg_idesc(kFmt, kPgKeys, false) | negate;
+    const uint32_t idesc = pg_idesc(kFmt, kPgHalf, false) | negate;
+    const uint32_t idesc_whole = pg_idesc(kFmt, kPgKeys, false) | negate;
     const uint64_t desc = tc_desc(0, 16);
     const bool leader = pg_elect();
     int r = kRing - 2, phase = 1;  // ring slot and phase parity of the newest K
@@ -707,28 +724,28 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         }
       } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll 1
-        for (int t = 0; t < many; ++t) {
-          const int s = (n + t) & 1;
-          // the buffer is free once the product of two steps ago has read its probabilities
-          if (n + t >= 2 && !pg_warp_wait(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
-            failed = true;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t qd = desc + ((t ? rec1 : rec) >> 16);
-          if (leader) {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
-              tc_mma(s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+          for (int t = 0; t < many; ++t) {
+            const int s = (n + t) & 1;
+            // the buffer is free once the product of two steps ago has read its probabilities
+            if (n + t >= 2 && !pg_warp_wait(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
+              failed = true;
+              break;
             }
-            tc_commit(b_s + 8 * (2 * s + h));
+            tc_fence_after();
+            const uint64_t qd = desc + ((t ? rec1 : rec) >> 16);
+            if (leader) {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = (kk >> 2) * (kBox >> 4) + (kk & 3) * 2;
+                tc_mma(s * 128 + h * kPgHalf, qd + off, kd + off + h * (kPgHalf * 128 >> 4), idesc, kk > 0);
+              }
+              tc_commit(b_s + 8 * (2 * s + h));
+            }
           }
+          if (failed) break;
         }
-        if (failed) break;
-      }
       }
       if (failed) break;
       if (leader) {
@@ -995,11 +1012,16 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
   grid_dependency_wait();
   allow_dependents();
   // ---- where the partials are: CTAs [c.x, c.y] of the prefix unit and of the own unit (bounds are
-  // read beside the length, before it is known whether they count)
+  // read beside the length, before it is known whether they count; kept within the grid, since a
+  // CTA that gave up on a wait leaves them unwritten)
   const int len = paged_len(A, b);
   const int tile = b / A.per_tile, grp = tile >> 1, unit = b * A.heads_kv + h;
   const int unit_p = h * ((A.tiles + 1) / 2) + grp;
-  const int2 cp = A.shared > 0 ? A.bounds[unit_p] : make_int2(0, -1), co = A.bounds[A.units + unit];
+  auto held = [&](int2 c) {
+    c.x = imax(0, imin(c.x, A.ctas - 1));
+    return make_int2(c.x, imax(c.x, imin(c.y, A.ctas - 1)));
+  };
+  const int2 cp = A.shared > 0 ? held(A.bounds[unit_p]) : make_int2(0, 0), co = held(A.bounds[A.units + unit]);
   const bool has_p = A.shared > 0 && len >= A.shared, has_o = paged_own_chunks(A, len) > 0;
   const bool pair = 2 * grp + 1 < A.tiles;
   const int subs = pair ? 1 : 2, sub0 = pair ? tile & 1 : 0;  // streams of a prefix piece with this tile
