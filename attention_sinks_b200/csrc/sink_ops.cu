@@ -384,7 +384,8 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
                       (kv->pages == 1 || (kv->k_stride_p >= D && kv->v_stride_p >= D));
   if (!q_rows || !k_rows) return SINK_ELAYOUT;
   if (!std::isfinite(scale)) return SINK_EINVAL;
-  // chunks of all sequences together stay in int
+  // a sequence's rows, rounded up to a chunk, and the chunks of all sequences together stay in int
+  if (int64_t(kv->table_width) * page > INT_MAX - kPgKeys) return SINK_EINVAL;
   if (int64_t(kv->batch) * ((int64_t(kv->table_width) * page + kPgKeys - 1) / kPgKeys) > INT_MAX) return SINK_EINVAL;
   if (!workspace || workspace_bytes < 256 || !aligned16(workspace)) return SINK_EWORKSPACE;
   int dev = 0;

@@ -446,11 +446,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(b_s + 8 * i, 1);
-      mbar_init(b_p + 8 * i, 128);
+      mbar_init(b_p + 8 * i, 4);
       mbar_init(b_pv + 8 * i, 1);
       mbar_init(b_rec + 8 * i, 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(b_wg + 8 * i, 128);
+    for (int i = 0; i < 2; ++i) mbar_init(b_wg + 8 * i, 4);
     mbar_init(b_done, 2);
     *flag = 0;
     start[0] = A.batch;
@@ -558,30 +558,44 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   bool failed = false;
   const bool narrow_prefix = A.tiles == 1 && A.batch * A.group <= kPgNarrow;
   if (warp == kPgLoadWarp) {
-    // ================================================================ loads (the warp's lanes share a tile's pages)
-    const int npg = kPgKeys / A.page_size;
+    // ================================================================ loads (a lane per page of a tile)
+    // The warp's own instructions bound a chunk that is in L2: with divisions by the ring's and the
+    // pages' sizes and a wait per tile 0.99 us at D = 64, without 0.87 (0.74 is memory's rate), and
+    // 1.16 in place of 1.27 at D = 128.  A second warp for V made 64 sequences with 4K shared rows
+    // 45.2 us in place of 43.4.  Where the ring holds whole chunks one vote waits for both tiles;
+    // an odd ring keeps K and V apart, not to leave its last slot empty.
+    constexpr bool kBoth = kRing % 2 == 0;
+    const int npg = kPgKeys / A.page_size, page_bits = 31 - __clz(A.page_size);
     const int qrow_bytes = A.group * 128 * kBoxes;
-    int tile = 0, step = 0;    // ring tiles and steps issued
-    int wide = 0, thin = 0;    // wide and narrow Q tiles issued
-    auto ring_slot = [&](int i) -> bool {  // waits until tile i's slot is free
-      return i < kRing || pg_warp_wait(b_empty + 8 * (i % kRing), ((i / kRing) - 1) & 1);
+    const uint32_t box_rows = lane * A.page_size * 128;  // this lane's page within a box
+    int slot_k = 0, slot_v = 1;                // ring slots of the next K and V,
+    uint32_t phase_k = 1, phase_v = 1;         // and the parity of their release
+    int tile = 0, step = 0;            // ring tiles and steps issued
+    int wide = 0, thin = 0;            // wide and narrow Q tiles issued
+    // An own piece reads its rows through its own row of the table, the shared ones (the prefix's,
+    // or a shorter sequence's) through row 0.  `row0`, `limit`: this lane's first row of chunk 0,
+    // and where the rows end.
+    struct Rows {
+      const int32_t* table;
+      int row0, limit;
     };
-    // This lane's page of chunk j of a piece, -1 where its rows are past the end.  An own piece
-    // reads its rows through its own row of the table, the shared ones (the prefix's, or a
-    // shorter sequence's) through row 0.
-    auto row_of = [&](const PagedPiece& p, int j) -> int {  // this lane's first row, or -1
-      const int row = (p.own ? paged_own_row(A, p.len) : 0) + j * kPgKeys + lane * A.page_size;
-      return lane < npg && row < (p.own ? p.len : A.shared) ? row : -1;
+    auto rows_of = [&](const PagedPiece& p) {
+      const int own_row = p.own ? paged_own_row(A, p.len) : 0;
+      return Rows{A.table + (p.own && own_row == A.shared ? p.which * A.table_sb : 0), own_row + lane * A.page_size,
+                  lane >= npg ? 0 : p.own ? p.len : A.shared};
     };
-    auto page_of = [&](const PagedPiece& p, int j) -> int {
-      const int row = row_of(p, j);
-      if (row < 0) return -1;
-      return A.table[(p.own && paged_own_row(A, p.len) == A.shared ? p.which * A.table_sb : 0) + row / A.page_size];
+    // This lane's page of chunk j, -1 where its rows are past the end.
+    auto page_of = [&](const Rows& w, int j) -> int {
+      const int row = w.row0 + j * kPgKeys;
+      return unsigned(row) < unsigned(w.limit) ? w.table[row >> page_bits] : -1;
     };
     PagedPiece pc, ahead;
     bool live = walk.next(A, L, pc), more = false;
-    int page = live ? page_of(pc, pc.j0) : -1;
-    for (; live && !failed; live = more, pc = ahead) {
+    Rows rows{A.table, 0, 0}, rows_ahead = rows;
+    if (live) rows = rows_of(pc);
+    int page = live ? page_of(rows, pc.j0) : -1;
+    for (; live && !failed; live = more, pc = ahead, rows = rows_ahead) {
+      uint32_t q_bits[2] = {0, 0};
       const bool narrow = pc.own || narrow_prefix;
       if (lane == 0) {
         int* bound = reinterpret_cast<int*>(A.bounds + (pc.own ? A.units : 0) + pc.unit);
@@ -593,9 +607,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           failed = !pg_warp_wait(b_qempty + 8 * (i & 1), (i >> 1) & 1);
         wide = 0;
       }
-      const int nq = pc.pair ? 2 : 1;
-      uint32_t q_bits[2] = {0, 0};
-      for (int t = 0; t < nq && !failed; ++t) {
+      for (int t = 0; t < (pc.pair ? 2 : 1) && !failed; ++t) {
         const int slot = narrow ? 2 + (thin & 3) : wide & 1, use = narrow ? thin >> 2 : wide >> 1;
         if (use > 0 && !pg_warp_wait(b_qempty + 8 * slot, (use - 1) & 1)) {
           failed = true;
@@ -608,28 +620,36 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         __syncwarp();
         if (lane < copies * kBoxes) {  // a lane per copy
           const int x = lane / copies, c = lane - x * copies;
-          tma_load_3d(dst + x * kBox + c * 32 * 128,
-                      pc.own ? &A.qgroup : &A.qtile, 64 * x, pc.h * A.group,
+          tma_load_3d(dst + x * kBox + c * 32 * 128, pc.own ? &A.qgroup : &A.qtile, 64 * x, pc.h * A.group,
                       pc.own ? pc.which : (pc.which + t) * A.per_tile, bar);
         }
         q_bits[t] = uint32_t(slot) << 8 | uint32_t(use & 1) << 12 | (dst >> 4) << 16;
         narrow ? ++thin : ++wide;
       }
       more = walk.next(A, L, ahead);
-      const int first_page = more ? page_of(ahead, ahead.j0) : -1;  // in flight under this piece's chunks
+      if (more) rows_ahead = rows_of(ahead);
+      const int first_page = more ? page_of(rows_ahead, ahead.j0) : -1;  // in flight under this piece's chunks
       for (int j = pc.j0; j < pc.j1 && !failed; ++j) {
-        const int next_page = j + 1 < pc.j1 ? page_of(pc, j + 1) : first_page;
+        const int next_page = j + 1 < pc.j1 ? page_of(rows, j + 1) : first_page;
+        const int nq = pc.pair ? 2 : 1;
+        if (kBoth && !__all_sync(kFull, mbar_wait_bounded(b_empty + 8 * slot_k, phase_k) &&
+                                            mbar_wait_bounded(b_empty + 8 * slot_v, phase_v))) {
+          failed = true;
+          break;
+        }
         int at = page;
         if (at < 0 || at >= A.pages) {  // one past the pool: the copy reads zeros
           at = A.pages;
-          if (row_of(pc, j) >= 0) atomicOr(A.status, 2);
+          if (unsigned(rows.row0 + j * kPgKeys) < unsigned(rows.limit)) atomicOr(A.status, 2);
         }
+#pragma unroll
         for (int v = 0; v < 2; ++v, ++tile) {
-          if (!ring_slot(tile)) {
+          const int r = v ? slot_v : slot_k;
+          if (!kBoth && !pg_warp_wait(b_empty + 8 * r, v ? phase_v : phase_k)) {
             failed = true;
             break;
           }
-          const uint32_t bar = b_full + 8 * (tile % kRing), dst = s_ring + (tile % kRing) * kTB;
+          const uint32_t bar = b_full + 8 * r, dst = s_ring + r * kTB + box_rows;
           if (lane == 0) {
             if (v == 0) {  // the chunk's steps, published by the arrival
               const uint32_t ends = (j + 1 == pc.j1 ? PgStep::kQRelease : 0u) | (j == pc.j0 ? PgStep::kQWait : 0u);
@@ -645,21 +665,22 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           }
           __syncwarp();
           if (lane < npg) {
-            const CUtensorMap* map = v ? &A.vmap : &A.kmap;
-            for (int x = 0; x < kBoxes; ++x)
-              tma_load_4d(dst + x * kBox + lane * A.page_size * 128, map, 64 * x, 0, pc.h, at, bar);
+#pragma unroll
+            for (int x = 0; x < kBoxes; ++x) tma_load_4d(dst + x * kBox, v ? &A.vmap : &A.kmap, 64 * x, 0, pc.h, at, bar);
           }
         }
+        if ((slot_k += 2) >= kRing) slot_k -= kRing, phase_k ^= 1;
+        if ((slot_v += 2) >= kRing) slot_v -= kRing, phase_v ^= 1;
         step += nq;
         page = next_page;
       }
     }
     if (!failed) {  // tell the MMA warps that the steps end here
-      if (!ring_slot(tile)) {
+      if (!pg_warp_wait(b_empty + 8 * slot_k, phase_k)) {
         failed = true;
       } else if (lane == 0) {
         steps[step % kPgSteps] = PgStep::kStop;
-        mbar_arrive(b_full + 8 * (tile % kRing));
+        mbar_arrive(b_full + 8 * slot_k);
       }
     }
     if (failed) {  // let the copies in flight land before the CTA can exit (bounded waits)
@@ -818,8 +839,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + kPgO + s * 128 + lanes;
     const uint64_t scale2 = pg_pair(A.scale_log2, A.scale_log2);
     int step = 0, chunk = 0, syncs = 0;  // steps and chunks before this piece; barriers of the warpgroup
-    auto wg_sync = [&]() -> bool {       // the warpgroup's threads, bounded
-      mbar_arrive(b_wg + 8 * s);
+    auto arrive = [&](uint32_t bar) {  // the warp's, once every lane is here
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto wg_sync = [&]() -> bool {  // the warpgroup's threads, bounded
+      arrive(b_wg + 8 * s);
       return pg_warp_wait(b_wg + 8 * s, (syncs++) & 1);
     };
     // whether prefix row r of tile `tile` belongs to a sequence that has the whole prefix
@@ -886,8 +911,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           }
           tc_wait_st();
           tc_fence_before();
-          mbar_arrive(b_p + 16 * s);
-          mbar_arrive(b_p + 16 * s + 8);
+          arrive(b_p + 16 * s);
+          arrive(b_p + 16 * s + 8);
           continue;
         }
 #pragma unroll 1
@@ -911,7 +936,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             tc_wait_st();
           }
           tc_fence_before();
-          mbar_arrive(b_p + 16 * s + 8 * h);
+          arrive(b_p + 16 * s + 8 * h);
         }
       }
       const size_t slot = size_t(int(blockIdx.x) + pc.unit) * 2 + t;
