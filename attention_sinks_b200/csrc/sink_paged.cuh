@@ -94,18 +94,20 @@ struct PagedArgs {
 
 // ------------------------------------------------------------------ the line of work
 
-// Costs of a chunk in units of 64 clocks of one SM, by measurement: one tile or a pair of tiles on
-// it, and an own chunk, at least kOwnMin and, where memory bounds the own work, its share of the
-// time that memory takes for all of it (kOwnMem when every SM streams); kUnit for each own unit,
-// its query and the join of its result.  (Without kUnit the CTAs of one-chunk units finish last: 64
-// sequences with 4K shared and 32 own rows 44.5 us without, 43.2 with 14, 44.4 with 30, 45.5 with
-// 40; 64 sequences of 512 own rows, units all alike, 46.0 without and 46.7 with 14.)
+// Costs of a chunk in units of 64 clocks of one SM, by measurement (only their ratios count): one
+// tile or a pair of tiles on it, and an own chunk, at least kOwnMin and, where memory bounds the own
+// work, its share of the time that memory takes for all of it (kOwnMem when every SM streams); kUnit
+// for each own unit, its query and the join of its result.  (Without kUnit the CTAs of short units
+// finish last: 64 sequences with 4K shared and 16 to 1020 own rows 44.5 us without, 43.2 with 14,
+// 44.4 with 30, 45.5 with 40; 64 sequences of 512 own rows, units all alike, 46.0 without and 46.7
+// with 14.  A pair at 70 and 58 (D = 128, 64): 43.2 us, 42.0 at 80 and 62, 42.0 at 90 and 68, the
+// same with 16K shared and 512 own rows 56.5, 57.5, 61.3.)
 template <int D>
 struct PgCost {
-  static constexpr int kPair = D == 128 ? 70 : 58;
-  static constexpr int kOne = D == 128 ? 38 : 32;
-  static constexpr int kOwnMin = D == 128 ? 34 : 27;
-  static constexpr int kOwnMem = D == 128 ? 43 : 28;
+  static constexpr int kPair = D == 128 ? 80 : 62;
+  static constexpr int kOne = D == 128 ? 43 : 34;
+  static constexpr int kOwnMin = D == 128 ? 34 : 25;
+  static constexpr int kOwnMem = D == 128 ? 43 : 26;
   static constexpr int kUnit = 14;
 };
 
@@ -666,7 +668,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           __syncwarp();
           if (lane < npg) {
 #pragma unroll
-            for (int x = 0; x < kBoxes; ++x) tma_load_4d(dst + x * kBox, v ? &A.vmap : &A.kmap, 64 * x, 0, pc.h, at, bar);
+            for (int x = 0; x < kBoxes; ++x)
+              tma_load_4d(dst + x * kBox, v ? &A.vmap : &A.kmap, 64 * x, 0, pc.h, at, bar);
           }
         }
         if ((slot_k += 2) >= kRing) slot_k -= kRing, phase_k ^= 1;
