@@ -426,7 +426,8 @@ typedef struct sink_paged_kv {
  * Append: the first counts[b] tokens of k_new / v_new [batch, heads_kv, n, head_dim] become rows
  * lens[b] - counts[b] .. lens[b] - 1 of sequence b, k rotated to its position on the way (rot
  * NULL: as it is).  counts: device int32 [batch] (more than n counts as n), NULL for n
- * everywhere.  Tokens from counts[b] on, and tokens whose position is negative (an idle sequence: lens 0), are not written.
+ * everywhere.  Tokens from counts[b] on, and tokens whose position is negative (an idle
+ * sequence: lens 0), are not written.
  * q / q_out (both or neither; [batch, heads, n, head_dim]): rotated to the same positions in the
  * same launch, zeros for tokens that are not written.  Two sequences that append to one slot
  * leave one of the two rows there.
@@ -450,7 +451,7 @@ size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads
  * queries; a sequence of fewer rows attends to its own number of them.  shared_len is a
  * multiple of page_size, 0 for plain paged decode.  bf16 or fp16; head_dim 64 or 128;
  * page_size 16, 32, 64 or 128; 1 to 8 query heads per kv head; page, head and q rows 16-byte
- * aligned.
+ * aligned; table_width * page_size at most 2^31 - 129.
  */
 int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, int32_t shared_len,
                              float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,

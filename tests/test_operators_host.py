@@ -33,6 +33,7 @@ def attention(lib, kv, q=None, shared=0, out=P, sb=256, sh=64, ws=P, nbytes=1 <<
     (dict(status=None), _lib.EINVAL), (dict(batch=0), _lib.EINVAL), (dict(pages=0), _lib.EINVAL),
     (dict(table_width=0), _lib.EINVAL), (dict(page_size=0), _lib.EINVAL), (dict(page_size=48), _lib.EINVAL),
     (dict(page_size=128, table_width=1 << 26), _lib.EINVAL), (dict(dtype=_lib.DTYPE_F32), _lib.EDTYPE),
+    (dict(page_size=16, table_width=(1 << 27) - 1), _lib.EINVAL),  # rows end less than a chunk before 2^31
     (dict(dtype=9), _lib.EDTYPE), (dict(dtype=_lib.DTYPE_F16), _lib.EDTYPE), (dict(head_dim=96), _lib.EHEADDIM),
     (dict(head_dim=256), _lib.EHEADDIM), (dict(heads_kv=3), _lib.EGROUP), (dict(heads_kv=8), _lib.EGROUP),
     (dict(k=P + 2), _lib.ELAYOUT), (dict(v_stride_p=2044), _lib.ELAYOUT), (dict(k_stride_h=-1024), _lib.ELAYOUT),
