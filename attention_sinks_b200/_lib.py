@@ -547,20 +547,8 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-class on_device:
-    """Make device `index` current for the block; nothing to do when it is."""
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def current_device() -> int:
+    return torch._C._cuda_getDevice()
 
 
 def paged_workspace_bytes(batch: int, heads_kv: int, heads_q: int, head_dim: int, shared_len: int,

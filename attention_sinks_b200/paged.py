@@ -25,6 +25,12 @@ import torch
 from . import _lib
 from .rope import device_frequencies, rotation
 
+
+def _no_gradients() -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError("the paged cache keeps no gradients: call it under torch.no_grad() or detach its inputs")
+
+
 def _scratch(nbytes: int, index: int, stream: int) -> torch.Tensor:
     """Scratch of `attend`, one buffer per (thread, device, stream): a call's two launches follow
     each other on their stream, so one thread's calls there can share one; another thread's
@@ -138,11 +144,6 @@ class PagedKVCache:
             raise ValueError(f"{name} is [{self.batch}, {heads or 'Hq'}, {tokens}, {self.head_dim}] {self.dtype} on "
                              f"{self.device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
 
-    @staticmethod
-    def _no_gradients(*tensors: torch.Tensor | None) -> None:
-        if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
-            raise RuntimeError("the paged cache keeps no gradients: call it under torch.no_grad() or detach its inputs")
-
     def append(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                counts: torch.Tensor | None = None) -> torch.Tensor | None:
         """Store the first counts[b] (all, when None) of the tokens k, v [B, Hkv, T, D] as the last
@@ -151,7 +152,11 @@ class PagedKVCache:
         Tokens from counts[b] on, and all of an idle sequence's (lens 0), are not stored; their
         q rows come back as zeros.  counts: int32 [B] on the device.  Sequences may share pages that
         they read; of two that append to one slot, one row stays."""
-        self._no_gradients(k, v, q)
+        if _lib.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.append(k, v, q, counts)
+        if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+            _no_gradients()
         form = (self._like, _lib.form_of(k), _lib.form_of(v), _lib.form_of(q), _lib.form_of(counts))
         known = _lib.forms("append")
         call = known.get(form)
@@ -162,12 +167,11 @@ class PagedKVCache:
         q_out = None if q is None else torch.empty_like(q)
         if call.empty:
             return q_out
-        with _lib.on_device(self._index):
-            rc = _lib.lib().sink_paged_append(self._kv_ref, call.k.at(k), call.v.at(v),
-                                              None if counts is None else counts.data_ptr(),
-                                              None if q is None else call.q.at(q),
-                                              None if q is None else call.q_out.at(q_out), self._rot_ref,
-                                              _lib.raw_stream(self._index))
+        rc = _lib.lib().sink_paged_append(self._kv_ref, call.k.at(k), call.v.at(v),
+                                          None if counts is None else counts.data_ptr(),
+                                          None if q is None else call.q.at(q),
+                                          None if q is None else call.q_out.at(q_out), self._rot_ref,
+                                          _lib.raw_stream(self._index))
         if rc:
             _lib._check(rc, "sink_paged_append")
         return q_out
@@ -181,7 +185,11 @@ class PagedKVCache:
         sequences: they are read through the first row of the block table, once per kv head
         for the whole batch.  bfloat16 or float16, head_dim 64 or 128, pages of 16, 32, 64 or
         128 rows, up to 8 query heads per kv head."""
-        self._no_gradients(q)
+        if _lib.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attend(q, scale, shared_len)
+        if q.requires_grad:
+            _no_gradients()
         aligned = q.data_ptr() % 16 == 0
         form = (self._like, _lib.form_of(q), shared_len, aligned)
         known = _lib.forms("attend")
@@ -193,13 +201,12 @@ class PagedKVCache:
         out = q.new_empty(call.shape)
         if self.batch == 0:
             return out
-        with _lib.on_device(self._index):
-            stream = _lib.raw_stream(self._index)
-            work = _scratch(call.workspace, self._index, stream)
-            rc = _lib.lib().sink_paged_attention(call.q.at(q), self._kv_ref, shared_len,
-                                                 self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
-                                                 call.shape[2] * self.head_dim, self.head_dim, work.data_ptr(),
-                                                 work.numel(), stream)
+        stream = _lib.raw_stream(self._index)
+        work = _scratch(call.workspace, self._index, stream)
+        rc = _lib.lib().sink_paged_attention(call.q.at(q), self._kv_ref, shared_len,
+                                             self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                                             call.shape[2] * self.head_dim, self.head_dim, work.data_ptr(),
+                                             work.numel(), stream)
         if rc:
             _lib._check(rc, "sink_paged_attention")
         return out
@@ -208,7 +215,7 @@ class PagedKVCache:
         """Raise RuntimeError if a kernel met a position past the block table or a page outside
         the pool since the last check (nothing was accessed there); synchronises the stream."""
         st = ctypes.c_int32(0)
-        with _lib.on_device(self._index):
+        with torch.cuda.device(self._index):
             _lib._check(_lib.lib().sink_read_status(self.status.data_ptr(), _lib.raw_stream(self._index),
                                                     ctypes.byref(st)), "sink_read_status")
         _lib.raise_status(st.value)

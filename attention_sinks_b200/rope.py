@@ -164,6 +164,9 @@ class _RotaryCall:
         self.rot_ref = ctypes.byref(self.rot)
 
     def __call__(self, q, k, positions, inv_freq, interleaved, scale, inverse):
+        if _lib.current_device() != self.index:
+            with torch.cuda.device(self.index):
+                return self(q, k, positions, inv_freq, interleaved, scale, inverse)
         if self.copy_q:
             q = q.contiguous()
         if self.copy_k:
@@ -178,11 +181,10 @@ class _RotaryCall:
             inv_freq = device_frequencies(inv_freq, self.device)
         rot = self.rot
         rot.inv_freq, rot.interleaved, rot.scale, rot.inverse = inv_freq.data_ptr(), interleaved, scale, inverse
-        with _lib.on_device(self.index):
-            rc = _lib.lib().sink_rotary(self.batch, self.dim, self.q.at(q), self.q_out.at(q_out),
-                                        None if k is None else self.k.at(k),
-                                        None if k is None else self.k_out.at(k_out), positions.data_ptr(),
-                                        self.pos_stride, self.rot_ref, _lib.raw_stream(self.index))
+        rc = _lib.lib().sink_rotary(self.batch, self.dim, self.q.at(q), self.q_out.at(q_out),
+                                    None if k is None else self.k.at(k),
+                                    None if k is None else self.k_out.at(k_out), positions.data_ptr(),
+                                    self.pos_stride, self.rot_ref, _lib.raw_stream(self.index))
         if rc:
             _lib._check(rc, "sink_rotary")
         return q_out, k_out
