@@ -33,6 +33,14 @@
 // warp idle.  Such a narrow tile holds its rows four times, 32 lanes apart, and warp w of the
 // warpgroup takes the w-th quarter of the keys, probability 0 elsewhere; the four partial
 // results are joined at the end of the piece.
+//
+// Measured, against the rate of a plain copy (6.5 TB/s) and of a library product (1672 TFLOP/s):
+// 64 sequences of 16K own rows, 8 kv heads, D = 64: 333 us, 6.4 TB/s; of 1K to 16K rows, D = 128:
+// 374 to 418 us, 5.6 to 6.3 TB/s.  A prefix of 32K rows for 64 sequences of 4 query heads per kv
+// head, D = 128: 49 us, 700 TFLOP/s; for 256, D = 64: 131 us, 520 TFLOP/s, bound by the
+// exponentials (53 % of the special-function rate) and the wait for the products between them.
+// 4K shared and 16 to 1020 own rows, 64 sequences: 42 us for 23 us of bytes, 8 us of it start
+// and join.
 #pragma once
 
 #include <cuda.h>
@@ -1027,7 +1035,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
 // weights 2^(m - max m) of each row's partials (prefix pieces, then own pieces, in line order,
 // two streams each), then the weighted sums, 16 bytes of a row per thread.  Where a row has
 // fewer words than the CTA threads, teams of threads share its partials and their sums are
-// added in team order: the result does not depend on scheduling.
+// added in team order: the result does not depend on scheduling.  Bound by the latency of
+// three dependent reads (bounds, maxima, words): 4 us for 512 CTAs, 12 us for 2048, in part under
+// the attention's tail.
 constexpr int kPgCombineThreads = 256;
 
 template <typename T, int D>
