@@ -26,6 +26,8 @@ int elem_size(int32_t dt) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int64_t kPagedMaxRows = 1 << 24;  // batch * query heads: row indexes stay in int
+constexpr int64_t kPagedMaxChunks = 1 << 22;  // batch * kv heads * chunks of a table's row, per SM: the
+                                              // cost of a CTA's part stays below 2^29 (PagedWalk)
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -386,11 +388,13 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   if (!std::isfinite(scale)) return SINK_EINVAL;
   // a sequence's rows, rounded up to a chunk, and the chunks of all sequences together stay in int
   if (int64_t(kv->table_width) * page > INT_MAX - kPgKeys) return SINK_EINVAL;
-  if (int64_t(kv->batch) * ((int64_t(kv->table_width) * page + kPgKeys - 1) / kPgKeys) > INT_MAX) return SINK_EINVAL;
+  const int64_t chunks = int64_t(kv->batch) * ((int64_t(kv->table_width) * page + kPgKeys - 1) / kPgKeys);
+  if (chunks > INT_MAX) return SINK_EINVAL;
   if (!workspace || workspace_bytes < 256 || !aligned16(workspace)) return SINK_EWORKSPACE;
   int dev = 0;
   const int sms = device_sms(&dev);
   if (sms <= 0) return SINK_EDEVICE;
+  if (chunks * kv->heads_kv > sms * kPagedMaxChunks) return SINK_EINVAL;
   PagedPlan plan;
   if (!plan_paged(kv->batch, kv->heads_kv, q->heads, D, shared_len, sms, plan)) return SINK_EINVAL;
   if (workspace_bytes < plan.total) return SINK_EWORKSPACE;

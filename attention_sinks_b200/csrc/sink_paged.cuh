@@ -165,18 +165,17 @@ __device__ __forceinline__ int paged_own_chunks(const PagedArgs& A, int len) {
   return (len - paged_own_row(A, len) + kPgKeys - 1) / kPgKeys;
 }
 
-// Chunks [j0, j1) of the unit at `base`, n chunks of cost w after a cost u (u + n * w < 2^32), that
-// start in [lo, hi).  The first starts at the base, the others behind u and those before them.
-__device__ __forceinline__ void paged_span(long long lo, long long hi, long long base, int n, int w, int u, int& j0,
-                                           int& j1) {
-  auto started = [&](long long x) -> int {  // chunks that start before x
+// Chunks [j0, j1) of the unit at `base`, n chunks of cost w after a cost u (u + n * w < 2^31), that
+// start in [0, span).  The first starts at the base, the others behind u and those before them.
+__device__ __forceinline__ void paged_span(int span, int base, int n, int w, int u, int& j0, int& j1) {
+  auto started = [&](int x) -> int {  // chunks that start before x
     if (x <= base) return 0;
-    const long long d = x - base;
-    if (d >= (long long)u + (long long)n * w) return n;
-    return d <= u + w ? 1 : int((unsigned(d) - unsigned(u) + unsigned(w) - 1) / unsigned(w));
+    const unsigned d = unsigned(x) - unsigned(base);
+    if (d >= unsigned(u) + unsigned(n) * unsigned(w)) return n;
+    return d <= unsigned(u + w) ? 1 : int((d - unsigned(u) + unsigned(w) - 1) / unsigned(w));
   };
-  j0 = started(lo);
-  j1 = started(hi);
+  j0 = started(0);
+  j1 = started(span);
 }
 
 struct PagedPiece {
@@ -189,14 +188,15 @@ struct PagedPiece {
   bool own, pair;
 };
 
-// Walks the pieces of one CTA in line order.  Every role of the CTA runs its own copy.
+// Walks the pieces of one CTA in line order, positions counted from the start of its part (the host
+// keeps a part below 2^29).  Every role of the CTA runs its own copy.
 struct PagedWalk {
-  long long lo, hi, base;
+  int span, base;        // length of the part; where the next unit starts
   int unit, h, at, len;  // at: group of the head, or sequence
   bool own;
 
   __device__ __forceinline__ bool next(const PagedArgs& A, const PagedLine& L, PagedPiece& p) {
-    while (base < hi) {
+    while (base < span) {
       int n, w, u = 0;
       if (!own) {
         if (unit >= L.units) {
@@ -231,8 +231,8 @@ struct PagedWalk {
         len = -1;
         continue;
       }
-      paged_span(lo, hi, base, n, w, u, p.j0, p.j1);
-      base += u + (long long)n * w;
+      paged_span(span, base, n, w, u, p.j0, p.j1);
+      base += u + n * w;
       ++unit;
       if (own) {
         if (++h == A.heads_kv) {
@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   before -= mine;
   const PagedLine L = paged_line<D>(A, int(all), int(all >> 32), prefix);
   PagedWalk walk;
-  walk.lo = L.per_cta * blockIdx.x;
-  walk.hi = walk.lo + L.per_cta < L.total ? walk.lo + L.per_cta : L.total;
+  const long long lo = L.per_cta * blockIdx.x, rest = L.total - lo;
+  walk.span = int(rest < 0 ? 0 : rest < L.per_cta ? rest : L.per_cta);
   walk.cost_pair = PgCost<D>::kPair;
   walk.cost_one = PgCost<D>::kOne;
   walk.unit_cost = PgCost<D>::kUnit;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     return ((n & 0xffffffffll) * L.own_cost + (n >> 32) * PgCost<D>::kUnit) * A.heads_kv;
   };
   if (mine > 0) {  // the sequence whose work holds position lo
-    const long long want = walk.lo - L.prefix_cost;
+    const long long want = lo - L.prefix_cost;
     if (want >= own_cost(before) && want < own_cost(before + mine)) {
       long long c = before;
       for (int b = b_lo; b < b_hi; ++b) {
@@ -541,26 +541,27 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // the CTA holds all 512 columns
   const uint32_t tmem_held = *tmem_slot;
-  if (walk.lo < L.prefix_cost) {
+  if (lo < L.prefix_cost) {
     walk.own = false;
     walk.len = 0;
-    walk.h = int(pg_div(walk.lo, L.head_cost));
-    const long long r = walk.lo - walk.h * L.head_cost;
+    walk.h = int(pg_div(lo, L.head_cost));
+    const long long r = lo - walk.h * L.head_cost;
     const long long pair_cost = (long long)L.chunks * PgCost<D>::kPair;
     walk.at = imin(int(pg_div(r, pair_cost)), L.groups - 1);  // the groups before the last are pairs
     walk.unit = walk.h * L.groups + walk.at;
-    walk.base = walk.h * L.head_cost + walk.at * pair_cost;
+    walk.base = int(walk.at * pair_cost - r);
   } else {
     walk.own = true;
     walk.at = start[0];
-    walk.base = L.prefix_cost + *reinterpret_cast<const long long*>(start + 2);
+    const long long into = lo - L.prefix_cost - *reinterpret_cast<const long long*>(start + 2);
+    walk.base = 0;
     walk.len = -1;
     walk.h = 0;
     if (walk.at < A.batch) {
       walk.len = start[1];
       const long long unit_cost = (long long)L.own_cost * paged_own_chunks(A, walk.len) + PgCost<D>::kUnit;
-      walk.h = int(pg_div(walk.lo - walk.base, unit_cost));
-      walk.base += walk.h * unit_cost;
+      walk.h = int(pg_div(into, unit_cost));
+      walk.base = int(walk.h * unit_cost - into);
     }
     walk.unit = walk.at * A.heads_kv + walk.h;
   }

@@ -451,7 +451,8 @@ size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads
  * queries; a sequence of fewer rows attends to its own number of them.  shared_len is a
  * multiple of page_size, 0 for plain paged decode.  bf16 or fp16; head_dim 64 or 128;
  * page_size 16, 32, 64 or 128; 1 to 8 query heads per kv head; page, head and q rows 16-byte
- * aligned; table_width * page_size at most 2^31 - 129.
+ * aligned; table_width * page_size at most 2^31 - 129; batch * heads_kv * the 128-row chunks of a
+ * table row at most 2^22 per SM of the device.
  */
 int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, int32_t shared_len,
                              float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
