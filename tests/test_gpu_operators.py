@@ -411,6 +411,20 @@ def test_paged_attention_refusals():
     cache.check_status()
 
 
+def test_paged_attention_refuses_tables_of_too_much_work():
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    heads = 64
+    width = sms * (1 << 22) // heads + 1  # one chunk of 128 rows per page, one more than 2^22 of them per SM
+    pools = torch.zeros(1, heads, 128, 64, device=DEV, dtype=BF)
+    table = torch.zeros(1, width, dtype=torch.int32, device=DEV)
+    lens = torch.ones(1, dtype=torch.int32, device=DEV)
+    q = randn(gen(28), 1, heads, 1, 64)
+    with pytest.raises(RuntimeError, match="sinkcache_b200"):
+        PagedKVCache(pools, pools.clone(), table, lens).attend(q)
+    out = PagedKVCache(pools, pools.clone(), table[:, :width - 1], lens).attend(q)
+    assert out.shape == (1, 1, heads, 64) and not out.any()
+
+
 def test_paged_calls_on_nothing():
     pools = torch.zeros(3, 2, 16, 64, device=DEV, dtype=BF)
     none = PagedKVCache(pools, pools.clone(), torch.zeros(0, 4, dtype=torch.int32, device=DEV),
