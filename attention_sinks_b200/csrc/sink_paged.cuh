@@ -409,6 +409,13 @@ __device__ __forceinline__ bool pg_half_step(uint32_t (&r)[N], int keys, bool va
   return true;
 }
 
+// A partial result's (maximum, sum).  A maximum of -infinity says that nothing is there, and is
+// what NaN scores leave too (fmaxf passes over them): their sum is NaN, so they count as a
+// partial with a maximum of 0, and the row's result is NaN.
+__device__ __forceinline__ float2 pg_partial(float mref, float l) {
+  return make_float2(mref == kNegInf && l != 0.f ? 0.f : mref, l);
+}
+
 // What the MMA warps have to know of a step, written by the load warp.
 struct PgStep {
   static constexpr uint32_t kFirst = 1u;                   // the piece's first step on its stream
@@ -965,7 +972,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           // the four warps' results over their keys, joined in shared memory
           float* part = reinterpret_cast<float*>(gbase + kTB + s * (G_::kMergeBytes / 2));  // [4][8][D]
           float2* ml = g_ml + s * 4 * kPgNarrow;
-          if (lane < rows) ml[wq * kPgNarrow + lane] = make_float2(mref, l);
+          if (lane < rows) ml[wq * kPgNarrow + lane] = pg_partial(mref, l);
 #pragma unroll
           for (int x = 0; x < D; x += 32) {
             uint32_t o[32];
@@ -1013,7 +1020,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             }
           }
           // a sequence without the whole prefix does not take part
-          if (counts) ml_to[row] = takes_part(tile, row) ? make_float2(mref, l) : make_float2(kNegInf, 0.f);
+          if (counts) ml_to[row] = takes_part(tile, row) ? pg_partial(mref, l) : make_float2(kNegInf, 0.f);
         }
         tc_fence_before();
       }
