@@ -410,6 +410,9 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   A.lens = kv->lens;
   A.status = kv->status;
   A.out = static_cast<char*>(out);
+  A.v = static_cast<const char*>(kv->v);
+  A.v_sp = kv->v_stride_p;
+  A.v_sh = kv->v_stride_h;
   A.table_sb = kv->table_stride;
   A.o_sb = out_stride_b;
   A.o_sh = out_stride_h;

@@ -91,6 +91,8 @@ struct PagedArgs {
   float2* ml_prefix; // [prefix slots][2][128] (maximum, sum)
   float* o_own;      // [own slots][2][G][D]
   float2* ml_own;
+  const char* v;     // the V pool, for the combine's look at values that are not finite
+  int64_t v_sp, v_sh;
   int2* bounds;      // first and last CTA with a piece of the unit: prefix units, then own units
   int units;         // prefix units that `bounds` has room for
   int batch, heads_kv, group, page_size, pages, table_width, shared;
@@ -1048,6 +1050,24 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
 // the attention's tail.
 constexpr int kPgCombineThreads = 256;
 
+// Which of NaN (bit 0), +infinity (1) and -infinity (2) the values of dims 4 x .. 4 x + 3 hold in
+// the rows [0, len) of sequence b, kv head h: 3 bits a dim.  By a whole warp, a row per lane.
+template <typename T, int D>
+__device__ __noinline__ unsigned pg_value_kinds(const PagedArgs& A, int b, int h, int len, int x) {
+  unsigned kinds = 0;
+  for (int r = threadIdx.x & 31; r < len; r += 32) {
+    const int page = (r < A.shared ? A.table : A.table + b * A.table_sb)[r / A.page_size];
+    if (page < 0 || page >= A.pages) continue;
+    const T* row = reinterpret_cast<const T*>(A.v) + page * A.v_sp + h * A.v_sh + r % A.page_size * D + 4 * x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float v = Elem<T>::to_f(row[k]);
+      kinds |= (isnan(v) ? 1u : !isinf(v) ? 0u : v > 0.f ? 2u : 4u) << (3 * k);
+    }
+  }
+  return __reduce_or_sync(kFull, kinds);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(const __grid_constant__ PagedArgs A) {
   extern __shared__ float w[];  // [G][parts], then the teams' sums
@@ -1139,11 +1159,29 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
       o.z += v.z;
       o.w += v.w;
     }
-    const float total = inv[g], r = total == 0.f ? 0.f : 1.f / total;
-    T* out = reinterpret_cast<T*>(A.out) + b * A.o_sb + (h * G + g) * A.o_sh + 4 * x;
-    const float y[4] = {o.x, o.y, o.z, o.w};
+  }
+  const float total = team == 0 ? inv[g] : 0.f, r = total == 0.f ? 0.f : 1.f / total;
+  float y[4] = {o.x * r, o.y * r, o.z * r, o.w * r};
+  // A narrow tile meets every value with the probability 0 of the warps whose key it is not, and 0
+  // times an infinity is NaN; so is it where a probability or weight that is not 0 rounds to 0.
+  // Where the sum of probabilities is a number, a NaN is taken back to what the values say: the
+  // infinity that is there, if it is of one sign and no NaN beside it.
+  const bool odd = total != 0.f && total == total && (y[0] != y[0] || y[1] != y[1] || y[2] != y[2] || y[3] != y[3]);
+  for (unsigned left = __ballot_sync(kFull, odd); left != 0; left &= left - 1) {
+    const int src = __ffs(left) - 1;
+    const unsigned kinds = pg_value_kinds<T, D>(A, b, h, len, __shfl_sync(kFull, x, src));
+    if (lane == src) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = Elem<T>::from_f(total == 0.f ? 0.f : y[k] * r);
+      for (int k = 0; k < 4; ++k) {
+        const unsigned kind = (kinds >> (3 * k)) & 7u;
+        if (y[k] != y[k] && (kind == 2u || kind == 4u)) y[k] = kind == 2u ? -kNegInf : kNegInf;
+      }
+    }
+  }
+  if (team == 0) {
+    T* out = reinterpret_cast<T*>(A.out) + b * A.o_sb + (h * G + g) * A.o_sh + 4 * x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = Elem<T>::from_f(total == 0.f ? 0.f : y[k]);
   }
 }
 

@@ -100,3 +100,37 @@ def test_a_nan_query_of_an_idle_sequence():
     q[0] = NAN
     want = check(cache, q, clean)
     assert not want[0].any()
+
+
+@pytest.mark.parametrize("batch,hq,hkv,d,shared", [(3, 4, 2, 128, 0), (3, 6, 2, 64, 0), (2, 8, 2, 64, 256),
+                                                   (33, 8, 2, 128, 256), (70, 8, 1, 64, 640)],
+                         ids=["own", "own of odd groups", "narrow prefix", "wide prefix", "pair of tiles"])
+@pytest.mark.parametrize("values", [(INF,), (-INF,), (INF, INF), (INF, -INF), (NAN, INF), (NAN,)],
+                         ids=["inf", "-inf", "two", "both signs", "with nan", "nan"])
+def test_values_that_are_not_finite(batch, hq, hkv, d, shared, values):
+    """An infinite value gives an infinite output in its dim, NaN only beside a NaN or one of the
+    other sign; once in the first rows, once in the last."""
+    g = gen(batch + d)
+    lens = [shared + 200 + (i * 37) % 300 for i in range(batch)]
+    cache = make_cache(g, lens, hkv, 64, d, shared=shared)
+    q = randn(g, batch, hq, 1, d)
+    clean = formula(cache, q, shared)
+    for n, value in enumerate(values):
+        put(cache.v_pages, cache, 1, 40 + 50 * n, hkv - 1, value, dim=7, shared=shared)
+        put(cache.v_pages, cache, 1, lens[1] - 1 - 33 * n, 0, value, dim=d - 1)
+    want = check(cache, q, clean, shared)
+    assert not torch.isfinite(want[1, 0, -1, 7]) and not torch.isfinite(want[1, 0, 0, d - 1])
+
+
+@pytest.mark.parametrize("shared", [0, 128])
+def test_an_infinite_value_of_small_probability(shared):
+    """A probability that its 16-bit type rounds to 0 still gives its infinity: scores about 30
+    below the largest, 2^-43."""
+    g = gen(5)
+    cache = make_cache(g, [200, 150], 1, 32, 64, torch.float16, shared=shared)
+    q = randn(g, 2, 2, 1, 64, dtype=torch.float16)
+    put(cache.k_pages, cache, 0, 70, 0, (q[0, 0, 0] * 240 / q[0, 0, 0].square().sum()), shared=shared)
+    put(cache.k_pages, cache, 0, 71, 0, 0.0, shared=shared)
+    clean = formula(cache, q, shared)
+    put(cache.v_pages, cache, 0, 71, 0, -INF, dim=11, shared=shared)
+    assert check(cache, q, clean, shared)[0, 0, 0, 11] == -INF
