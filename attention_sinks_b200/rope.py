@@ -20,6 +20,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -202,7 +203,7 @@ def _launch(q, k, positions, inv_freq, interleaved, scale, inverse):
 class _Rotary(torch.autograd.Function):
     """The rotation is linear and (up to the attention scaling) orthogonal, so its backward
     pass is the rotation of the gradients by the negative angles: the same kernel, and itself
-    differentiable."""
+    differentiable.  Tangents are rotated as their tensors are."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
@@ -221,25 +222,42 @@ class _Rotary(torch.autograd.Function):
             raise RuntimeError("the positions or frequencies of a rotary call were changed in place before its "
                                "backward pass")
         interleaved, scale, inverse = ctx.how
-        rest = (positions, inv_freq, interleaved, scale, not inverse)
-        if not torch.is_grad_enabled():  # no graph of the backward pass is asked for
-            if dq is None:
-                return None, (_launch(dk, None, *rest)[0] if dk is not None else None), None, None, None, None, None
-            dq, dk = _launch(dq, dk, *rest)
-        elif dq is not None and dk is not None:
-            dq, dk = _Rotary.apply(dq, dk, *rest)
-        elif dq is not None:
-            dq = _Rotary.apply(dq, None, *rest)
+        if dq is not None:
+            dq, dk = _turn(dq, dk, positions, inv_freq, interleaved, scale, not inverse)
         elif dk is not None:
-            dk = _Rotary.apply(dk, None, *rest)
+            dk = _turn(dk, None, positions, inv_freq, interleaved, scale, not inverse)[0]
         return dq, dk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, dq, *rest):  # of q alone, as `_turn` calls it
+        positions, inv_freq, *_ = ctx.kept
+        return _Rotary.apply(dq, None, positions, inv_freq, *ctx.how)
+
+
+def has_tangent(*xs: torch.Tensor | None) -> bool:
+    """Whether forward-mode differentiation follows one of xs."""
+    if forward_ad._current_level < 0:
+        return False
+    return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
+def _turn(q, k, positions, inv_freq, interleaved, scale, inverse):
+    """(q, k) rotated, differentiably where gradients or tangents are asked for."""
+    if has_tangent(q, k):  # a tensor at a time: one may have a tangent and the other not
+        rest = positions, inv_freq, interleaved, scale, inverse
+        return _Rotary.apply(q, None, *rest), None if k is None else _Rotary.apply(k, None, *rest)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _Rotary.apply(q, k, positions, inv_freq, interleaved, scale, inverse)
+        return out if k is not None else (out, None)
+    return _launch(q, k, positions, inv_freq, interleaved, scale, inverse)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
            interleaved: bool = False, attention_scaling: float = 1.0):
     """Rotate q [B, Hq, T, D] and k [B, Hkv, T, D] (or None) at `positions` ([T] or [B, T]) by
     the angles positions * inv_freq, in one kernel launch; returns (q_rot, k_rot), new tensors
-    in the layout of the inputs (k_rot None without k).  Differentiable in q and k.
+    in the layout of the inputs (k_rot None without k).  Differentiable in q and k, in reverse and
+    forward mode.
 
     The first 2 * len(inv_freq) dims are rotated, the rest copied.  Pairs are (i, i + half), or
     (2i, 2i + 1) with `interleaved`.  Angles are formed in float64, the rotation in float32 with
@@ -248,7 +266,4 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     Forward and backward can be captured into a CUDA graph, on torch's terms: no autograd graph
     of the same leaf tensors made outside the capture may be alive.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        out = _Rotary.apply(q, k, positions, inv_freq, interleaved, attention_scaling, False)
-        return out if k is not None else (out, None)
-    return _launch(q, k, positions, inv_freq, interleaved, attention_scaling, False)
+    return _turn(q, k, positions, inv_freq, interleaved, attention_scaling, False)

@@ -1,0 +1,56 @@
+"""Calls of the rotation and the paged cache that their documentation allows or refuses, one by
+one: forward-mode derivatives, changed attributes, sizes past 32 bits."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad as fw
+
+from attention_sinks_b200 import rope_frequencies, rotary
+from tests import op_reference as ref
+from tests.test_gpu_operators import BF, DEV, FP, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_rotary_tangents_match_the_formula(dtype):
+    g, f = gen(41), rope_frequencies(48)[0].to(DEV)
+    pos = torch.randint(0, 5000, (2, 21), generator=g, device=DEV)
+    q, k, tq, tk = (randn(g, 2, h, 21, 80, dtype=dtype) for h in (4, 2, 4, 2))
+    with fw.dual_level():
+        both = rotary(fw.make_dual(q, tq), fw.make_dual(k, tk), pos, f, attention_scaling=1.25)
+        one = rotary(q, fw.make_dual(k, tk), pos, f, attention_scaling=1.25)
+        assert fw.unpack_dual(one[0]).tangent is None
+        for got, x, t in ((both[0], q, tq), (both[1], k, tk), (one[1], k, tk)):
+            got = fw.unpack_dual(got)
+            for y, value in ((got.primal, x), (got.tangent, t)):
+                want = ref.rotate(value, pos, f, False, 1.25)
+                ref.assert_bounded(y, want, ref.rotate_bound(value, want, f, False, 1.25, dtype))
+
+
+def test_rotary_tangents_match_differences():
+    """The rotation is linear: (f(x + t) - f(x - t)) / 2 is the tangent but for fp32 rounding, of
+    x +- t (2^-24 of them, turned by two terms) and of each rotation (its own bound)."""
+    g, f = gen(42), rope_frequencies(8)[0].to(DEV)
+    pos = torch.arange(3, device=DEV) + 11
+    q, t = randn(g, 1, 2, 3, 8, dtype=FP), randn(g, 1, 2, 3, 8, dtype=FP)
+    with fw.dual_level():
+        got = fw.unpack_dual(rotary(fw.make_dual(q, t), None, pos, f)[0]).tangent
+    diff = (rotary(q + t, None, pos, f)[0] - rotary(q - t, None, pos, f)[0]) / 2
+    size = q.abs() + t.abs()
+    bound = 2 * 2.0 ** -24 * (size + size.roll(4, -1)).double()
+    for x in (q + t, q - t, t):
+        bound += ref.rotate_bound(x, ref.rotate(x, pos, f), f, False, 1.0, FP)
+    ref.assert_bounded(got, diff.double(), bound + 2.0 ** -24 * diff.abs())
+
+
+def test_rotary_gradient_of_a_tangent():
+    g, f = gen(43), rope_frequencies(64)[0].to(DEV)
+    pos = torch.arange(20, device=DEV)
+    q, t, w = (randn(g, 1, 2, 20, 64, dtype=FP) for _ in range(3))
+    t.requires_grad_(True)
+    with fw.dual_level():
+        got = fw.unpack_dual(rotary(fw.make_dual(q, t), None, pos, f)[0]).tangent
+        dt, = torch.autograd.grad(got, t, w)
+    want = ref.rotate(w, pos, f, sign=-1)
+    ref.assert_bounded(dt, want, ref.rotate_bound(w, want, f, False, 1.0, FP))

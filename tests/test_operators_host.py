@@ -133,3 +133,60 @@ def test_rope_frequencies():
     for bad in (dict(rot_dim=7), dict(rot_dim=0), dict(rot_dim=8, factor=0.5), dict(rot_dim=8, kind="other")):
         with pytest.raises(ValueError):
             rope_frequencies(**bad)
+
+
+@pytest.fixture
+def plain_launch(monkeypatch):
+    """rotary's launch by the plain formula, on bare values as a kernel sees them."""
+    from attention_sinks_b200 import rope
+    from tests import op_reference
+
+    def launch(q, k, positions, inv_freq, interleaved, scale, inverse):
+        bare = [None if x is None else torch.autograd.forward_ad.unpack_dual(x).primal.detach() for x in (q, k)]
+        return tuple(None if x is None else op_reference.rotate(x, positions, inv_freq, interleaved, scale,
+                                                                -1 if inverse else 1).to(x.dtype) for x in bare)
+
+    monkeypatch.setattr(rope, "_launch", launch)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "both"])
+def test_rotary_carries_tangents(plain_launch, which):
+    from torch.autograd import forward_ad as fw
+
+    from tests import op_reference
+    g = torch.Generator().manual_seed(1)
+    f, pos = rope_frequencies(8)[0], torch.arange(5) + 3
+    q, k, tq, tk = (torch.randn(2, h, 5, 12, generator=g, dtype=torch.float64) for h in (3, 1, 3, 1))
+    with fw.dual_level():
+        x = fw.make_dual(q, tq) if which != "k" else q
+        y = fw.make_dual(k, tk) if which != "q" else k
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                got = [fw.unpack_dual(z) for z in rotary(x, y, pos, f, True, 1.5)]
+            for z, value, tangent, there in zip(got, (q, k), (tq, tk), (which != "k", which != "q")):
+                torch.testing.assert_close(z.primal, op_reference.rotate(value, pos, f, True, 1.5))
+                if there:
+                    torch.testing.assert_close(z.tangent, op_reference.rotate(tangent, pos, f, True, 1.5))
+                else:
+                    assert z.tangent is None
+        alone, none = rotary(x, None, pos, f)
+        assert none is None and (fw.unpack_dual(alone).tangent is not None) == (which != "k")
+
+
+def test_rotary_tangents_of_gradients(plain_launch):
+    """Forward over reverse: |rotate(x)|^2 has the gradient 2 x, whose tangent is 2 t."""
+    from torch.autograd import forward_ad as fw
+    g = torch.Generator().manual_seed(2)
+    f, pos = rope_frequencies(8)[0], torch.arange(5)
+    q, k, t = (torch.randn(1, 2, 5, 8, generator=g, dtype=torch.float64) for _ in range(3))
+    q.requires_grad_(True), k.requires_grad_(True)
+    with fw.dual_level():
+        for create in (True, False):
+            a, b = rotary(fw.make_dual(q, t), k, pos, f)
+            dq, dk = torch.autograd.grad((a * a).sum() + (b * b).sum(), (q, k), create_graph=create)
+            torch.testing.assert_close(fw.unpack_dual(dq).tangent, 2 * t)
+            torch.testing.assert_close(dk.detach(), 2 * k.detach())
+            s = t.clone().requires_grad_(True)  # reverse over forward
+            got = fw.unpack_dual(rotary(fw.make_dual(q, s), None, pos, f)[0]).tangent
+            ds, = torch.autograd.grad((got * got).sum(), s)
+            torch.testing.assert_close(ds, 2 * t)
