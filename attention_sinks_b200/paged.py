@@ -21,14 +21,17 @@ graph of the step serves every later token.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .rope import device_frequencies, rotation
+from .rope import device_frequencies, has_tangent, rotation
 
 
-def _no_gradients() -> None:
-    if torch.is_grad_enabled():
-        raise RuntimeError("the paged cache keeps no gradients: call it under torch.no_grad() or detach its inputs")
+def _no_gradients(*inputs: torch.Tensor | None) -> None:
+    """Refuse inputs that gradients or tangents are asked of: the cache keeps neither."""
+    if (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs)) or has_tangent(*inputs):
+        raise RuntimeError("the paged cache keeps no gradients or tangents: call it under torch.no_grad() or detach "
+                           "its inputs (in forward mode, take their primals)")
 
 
 def _scratch(nbytes: int, index: int, stream: int) -> torch.Tensor:
@@ -155,8 +158,8 @@ class PagedKVCache:
         if _lib.current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.append(k, v, q, counts)
-        if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
-            _no_gradients()
+        if forward_ad._current_level >= 0 or k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+            _no_gradients(k, v, q)
         form = (self._like, _lib.form_of(k), _lib.form_of(v), _lib.form_of(q), _lib.form_of(counts))
         known = _lib.forms("append")
         call = known.get(form)
@@ -188,8 +191,8 @@ class PagedKVCache:
         if _lib.current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.attend(q, scale, shared_len)
-        if q.requires_grad:
-            _no_gradients()
+        if forward_ad._current_level >= 0 or q.requires_grad:
+            _no_gradients(q)
         aligned = q.data_ptr() % 16 == 0
         form = (self._like, _lib.form_of(q), shared_len, aligned)
         known = _lib.forms("attend")

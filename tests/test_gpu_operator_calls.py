@@ -7,7 +7,7 @@ from torch.autograd import forward_ad as fw
 
 from attention_sinks_b200 import rope_frequencies, rotary
 from tests import op_reference as ref
-from tests.test_gpu_operators import BF, DEV, FP, gen, randn
+from tests.test_gpu_operators import BF, DEV, FP, gen, make_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,19 @@ def test_rotary_gradient_of_a_tangent():
         dt, = torch.autograd.grad(got, t, w)
     want = ref.rotate(w, pos, f, sign=-1)
     ref.assert_bounded(dt, want, ref.rotate_bound(w, want, f, False, 1.0, FP))
+
+
+def test_the_paged_cache_refuses_tangents():
+    g = gen(44)
+    cache = make_cache(g, [40, 20], 2, 16, 64)
+    q, k = randn(g, 2, 4, 1, 64), randn(g, 2, 2, 1, 64)
+    with fw.dual_level():
+        for bad in (lambda: cache.attend(fw.make_dual(q, q)), lambda: cache.append(fw.make_dual(k, k), k),
+                    lambda: cache.append(k, fw.make_dual(k, k)),
+                    lambda: cache.append(k, k, q=fw.make_dual(q, q))):
+            with pytest.raises(RuntimeError, match="tangents"):
+                bad()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangents"):
+                bad()
+        want = cache.attend(q)  # a level alone is nothing to refuse
+        assert torch.equal(cache.attend(fw.unpack_dual(fw.make_dual(q, q)).primal), want)
