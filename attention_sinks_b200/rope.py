@@ -257,7 +257,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     """Rotate q [B, Hq, T, D] and k [B, Hkv, T, D] (or None) at `positions` ([T] or [B, T]) by
     the angles positions * inv_freq, in one kernel launch; returns (q_rot, k_rot), new tensors
     in the layout of the inputs (k_rot None without k).  Differentiable in q and k, in reverse and
-    forward mode.
+    forward mode, and not in inv_freq (one that asks for gradients is refused).
 
     The first 2 * len(inv_freq) dims are rotated, the rest copied.  Pairs are (i, i + half), or
     (2i, 2i + 1) with `interleaved`.  Angles are formed in float64, the rotation in float32 with
@@ -266,4 +266,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     Forward and backward can be captured into a CUDA graph, on torch's terms: no autograd graph
     of the same leaf tensors made outside the capture may be alive.
     """
+    if (inv_freq.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0
+                                                                  and has_tangent(inv_freq)):
+        raise RuntimeError("rotary is not differentiable in its frequencies: detach inv_freq (apply_rope follows them)")
     return _turn(q, k, positions, inv_freq, interleaved, attention_scaling, False)

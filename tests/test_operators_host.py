@@ -190,3 +190,17 @@ def test_rotary_tangents_of_gradients(plain_launch):
             got = fw.unpack_dual(rotary(fw.make_dual(q, s), None, pos, f)[0]).tangent
             ds, = torch.autograd.grad((got * got).sum(), s)
             torch.testing.assert_close(ds, 2 * t)
+
+
+def test_rotary_refuses_frequencies_that_ask_for_gradients(plain_launch):
+    from torch.autograd import forward_ad as fw
+    f, pos = rope_frequencies(8)[0], torch.arange(5)
+    q = torch.ones(1, 2, 5, 8, dtype=torch.float64)
+    learned = f.clone().requires_grad_(True)
+    for x in (q, q.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="frequencies"):
+            rotary(x, None, pos, learned)
+    with torch.no_grad():
+        torch.testing.assert_close(rotary(q, None, pos, learned)[0], rotary(q, None, pos, f)[0])
+    with fw.dual_level(), pytest.raises(RuntimeError, match="frequencies"):
+        rotary(q, None, pos, fw.make_dual(f, f))
