@@ -139,6 +139,22 @@ class PagedKVCache:
         self._index = device.index
         _lib.prepare_device(device)  # before any graph capture of this cache's steps
         self._like = (k_pages.dtype, batch, hkv, d, device)  # what a call's form depends on here
+        self._fixed = frozenset((*self.__dict__, "_fixed"))
+
+    _fixed = frozenset()  # names of the attributes that stay, once they are all there
+
+    # The kernels read the memory that the attributes had when the cache was made, and the attributes
+    # are what keeps it: they can be updated in place (`cache.lens += 1` too) and not replaced.
+    def __setattr__(self, name: str, value) -> None:
+        if name in self._fixed and value is not getattr(self, name):
+            raise AttributeError(f"{name} of a paged cache cannot be replaced: update it in place, or make another cache "
+                                 "over the new one")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name: str) -> None:
+        if name in self._fixed:
+            raise AttributeError(f"{name} of a paged cache cannot be removed")
+        super().__delattr__(name)
 
     def _check_rows(self, name: str, x: torch.Tensor, heads: int | None, tokens: int) -> None:
         if (x.dim() != 4 or x.shape[0] != self.batch or (heads is not None and x.shape[1] != heads)

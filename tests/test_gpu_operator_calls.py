@@ -70,3 +70,18 @@ def test_the_paged_cache_refuses_tangents():
                 bad()
         want = cache.attend(q)  # a level alone is nothing to refuse
         assert torch.equal(cache.attend(fw.unpack_dual(fw.make_dual(q, q)).primal), want)
+
+
+def test_the_paged_cache_keeps_its_tensors():
+    g = gen(45)
+    cache = make_cache(g, [40, 20], 2, 16, 64)
+    q = randn(g, 2, 4, 1, 64)
+    want = cache.attend(q)
+    for name in ("k_pages", "v_pages", "block_table", "lens", "status"):
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(cache, name, getattr(cache, name).clone())
+    cache.lens -= 1
+    want_less, bound = ref.attend(q, cache.k_pages, cache.v_pages, cache.block_table, cache.lens, 0.125)
+    ref.assert_bounded(cache.attend(q), want_less, bound)
+    cache.lens += 1
+    assert torch.equal(cache.attend(q), want)

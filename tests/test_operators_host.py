@@ -204,3 +204,22 @@ def test_rotary_refuses_frequencies_that_ask_for_gradients(plain_launch):
         torch.testing.assert_close(rotary(q, None, pos, learned)[0], rotary(q, None, pos, f)[0])
     with fw.dual_level(), pytest.raises(RuntimeError, match="frequencies"):
         rotary(q, None, pos, fw.make_dual(f, f))
+
+
+def test_attributes_of_a_paged_cache_cannot_be_replaced():
+    cache = PagedKVCache.__new__(PagedKVCache)  # attributes alone: a cache is made over CUDA tensors
+    lens = cache.lens = torch.tensor([3, 4], dtype=torch.int32)
+    cache.page_size = 16
+    cache._fixed = frozenset(cache.__dict__)
+    cache.lens += 1  # in place
+    assert cache.lens is lens and lens.tolist() == [4, 5]
+    with pytest.raises(AttributeError, match="in place"):
+        cache.lens = cache.lens + 1
+    with pytest.raises(AttributeError, match="in place"):
+        cache.page_size = 32
+    with pytest.raises(AttributeError, match="removed"):
+        del cache.lens
+    cache.name = "layer 3"  # a caller's own
+    cache.name = "layer 4"
+    del cache.name
+    assert cache.lens is lens and cache.page_size == 16
