@@ -520,6 +520,13 @@ def form_of(x: torch.Tensor | None):
     return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
 
 
+def int32(name: str, value: int) -> int:
+    """`value`, refused where a 32-bit argument of the C ABI cannot hold it (ctypes would cut it)."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"sinkcache_b200: {name} of {value} does not fit in 32 bits")
+    return value
+
+
 class RowsArg:
     """A sink_rows_t argument, described once (from any tensor of its form, a meta one too) and
     pointed at a tensor per call."""
@@ -528,7 +535,8 @@ class RowsArg:
         if t.dim() != 4 or t.stride(-1) != 1:
             raise ValueError(f"expected a [B, H, n, D] tensor with unit last stride, got {tuple(t.shape)} "
                              f"strides {t.stride()}")
-        self.rows = Rows(0, dtype_code(t.dtype), t.shape[1], t.shape[2], 0, t.stride(0), t.stride(1), t.stride(2))
+        self.rows = Rows(0, dtype_code(t.dtype), int32("heads", t.shape[1]), int32("tokens", t.shape[2]), 0, t.stride(0),
+                         t.stride(1), t.stride(2))
         self.ref = ctypes.byref(self.rows)
 
     def at(self, t: torch.Tensor):

@@ -74,6 +74,7 @@ class _AttendCall:
 
     def __init__(self, cache, q, shared_len, aligned):
         cache._check_rows("q", q, None, 1)
+        _lib.int32("shared_len", shared_len)
         b, hq, _, d = q.shape
         # the kernel's tiled copies start rows on 16-byte boundaries
         self.copy = (not aligned or q.stride(-1) != 1 or q.stride(0) % 8 or q.stride(1) % 8
@@ -107,13 +108,13 @@ class PagedKVCache:
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
             raise ValueError(f"pools are [pages, Hkv, page_size, D] of one shape and type, got {tuple(k_pages.shape)} "
                              f"{k_pages.dtype}, {tuple(v_pages.shape)} {v_pages.dtype}")
-        pages, hkv, page, d = k_pages.shape
+        pages, hkv, page, d = (_lib.int32("a pool's size", n) for n in k_pages.shape)
         for x in (k_pages, v_pages):
             if x.stride(-1) != 1 or (page > 1 and x.stride(-2) != d):
                 raise ValueError("pages need contiguous rows (stride[-2] == head_dim, stride[-1] == 1)")
         if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(-1) != 1:
             raise ValueError("block_table is an int32 [B, width] tensor with a unit last stride")
-        batch, width = block_table.shape
+        batch, width = (_lib.int32("a block table's size", n) for n in block_table.shape)
         if lens.shape != (batch,) or lens.dtype != torch.int32 or not lens.is_contiguous():
             raise ValueError(f"lens is a contiguous int32 [{batch}] tensor")
         if status is None:

@@ -147,7 +147,7 @@ class _RotaryCall:
             raise ValueError(f"inv_freq {tuple(inv_freq.shape)} is not one-dimensional, or rotates more than a head of "
                              f"{d} dims (at most 512)")
         self.device, self.index = device, device.index
-        self.batch, self.dim = b, d
+        self.batch, self.dim = _lib.int32("batch", b), d
         # what a call has to convert first
         self.copy_q = q.stride(-1) != 1
         self.copy_k = k is not None and k.stride(-1) != 1

@@ -85,3 +85,17 @@ def test_the_paged_cache_keeps_its_tensors():
     ref.assert_bounded(cache.attend(q), want_less, bound)
     cache.lens += 1
     assert torch.equal(cache.attend(q), want)
+
+
+def test_sizes_past_32_bits_are_refused_not_cut():
+    g = gen(46)
+    cache = make_cache(g, [40, 20], 2, 16, 64)
+    q = randn(g, 2, 4, 1, 64)
+    for shared in (1 << 32, (1 << 32) + 16, -(1 << 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            cache.attend(q, shared_len=shared)
+    many = randn(g, 2, 2, 1, 64).expand(2, 2, (1 << 32) + 1, 64)  # one row seen as 2^32 + 1
+    before = cache.v_pages.clone()
+    with pytest.raises(ValueError, match="32 bits"):
+        cache.append(many, many)
+    assert torch.equal(cache.v_pages.view(torch.int16), before.view(torch.int16))

@@ -223,3 +223,14 @@ def test_attributes_of_a_paged_cache_cannot_be_replaced():
     cache.name = "layer 4"
     del cache.name
     assert cache.lens is lens and cache.page_size == 16
+
+
+def test_sizes_past_32_bits_are_refused_not_cut():
+    for good in (0, -(1 << 31), (1 << 31) - 1):
+        assert _lib.int32("x", good) == good
+    for bad in (1 << 31, (1 << 32) + 16, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="32 bits"):
+            _lib.int32("x", bad)
+    for shape in ((1, 1, (1 << 32) + 1, 64), (1, (1 << 32) + 1, 1, 64)):
+        with pytest.raises(ValueError, match="32 bits"):
+            _lib.RowsArg(torch.empty(64, dtype=torch.bfloat16, device="meta").expand(shape))
