@@ -491,13 +491,17 @@ def v2_gather(kbuf: torch.Tensor, vbuf: torch.Tensor, n_sink: int, window: int, 
 
 
 def raise_status(status: int) -> None:
-    """Raise what the status bits of a paged cache say."""
+    """Raise what the status bits of a paged cache say, all of them."""
+    met = []
+    if status & STATUS_WAIT_TIMEOUT:
+        met.append("a bounded wait ran out; the results of the launches since the last check are void")
     if status & STATUS_BAD_PAGE:
-        raise RuntimeError("sinkcache_b200: a position past the block table or a page index outside the pool was "
-                           "met since the last check; it was not accessed, and the results that needed it are void")
-    if status:
-        raise RuntimeError(f"sinkcache_b200 kernel status 0x{status:x}: a bounded wait ran out; the results of the "
-                           "launches since the last check are void")
+        met.append("a position past the block table or a page index outside the pool was met since the last check; it "
+                   "was not accessed, and the results that needed it are void")
+    if status & ~(STATUS_WAIT_TIMEOUT | STATUS_BAD_PAGE):
+        met.append("unknown failure")
+    if met:
+        raise RuntimeError(f"sinkcache_b200 kernel status 0x{status:x}: {'; '.join(met)}")
 
 
 # Calls of these operators take a few microseconds on the GPU for a single token, so what a call

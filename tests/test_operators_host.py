@@ -234,3 +234,13 @@ def test_sizes_past_32_bits_are_refused_not_cut():
     for shape in ((1, 1, (1 << 32) + 1, 64), (1, (1 << 32) + 1, 1, 64)):
         with pytest.raises(ValueError, match="32 bits"):
             _lib.RowsArg(torch.empty(64, dtype=torch.bfloat16, device="meta").expand(shape))
+
+
+def test_every_status_bit_is_reported():
+    _lib.raise_status(0)
+    page, wait = "page index outside", "bounded wait ran out"
+    for status, there, absent in ((1, [wait], [page]), (2, [page], [wait]), (3, [page, wait], []),
+                                  (4, ["unknown"], [page, wait]), (7, [page, wait, "unknown"], [])):
+        with pytest.raises(RuntimeError, match=f"sinkcache_b200.*0x{status:x}") as e:
+            _lib.raise_status(status)
+        assert all(x in str(e.value) for x in there) and not any(x in str(e.value) for x in absent)
