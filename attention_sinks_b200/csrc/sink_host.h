@@ -18,6 +18,9 @@ int device_sms(int* dev_out);
 // cuTensorMapEncodeTiled, looked up once (nullptr when the driver has none).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
+// What sink_debug_fail_next_wait armed, (chunk << 32) | polls, or -1; disarms it.
+int64_t take_fail_next_wait();
+
 // One-time set-up of device `dev` for the paged attention (sink_ops.cu); outside captures.
 int32_t prepare_paged(int dev);
 

@@ -433,6 +433,9 @@ int32_t sink_paged_attention(const sink_rows_t* q, const sink_paged_kv_t* kv, in
   A.tiles = plan.tiles;
   A.ctas = sms;
   A.negate = scale < 0.f;
+  const int64_t inject = take_fail_next_wait();
+  A.wait_polls = inject < 0 ? kWaitPolls : int(inject & 0x7fffffff);
+  A.skip_tile = inject < 0 ? -1 : int(inject >> 32);
   // a scale of 0 (uniform weights) becomes the smallest normal number, so that a masked score
   // of -infinity stays one
   A.scale_log2 = std::fmax(std::fabs(scale) * kLog2e, 1.17549435e-38f);

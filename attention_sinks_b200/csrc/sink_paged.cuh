@@ -100,6 +100,8 @@ struct PagedArgs {
   int ctas;
   float scale_log2;  // of |scale|
   uint32_t negate;   // scale < 0: the MMA negates Q
+  int wait_polls;    // of each bounded wait (kWaitPolls unless a failure-detection test shortens it)
+  int skip_tile;     // failure-detection test hook, -1 when off: the K or V tile that no CTA loads (nor those behind it)
 };
 
 // ------------------------------------------------------------------ the line of work
@@ -278,9 +280,17 @@ __device__ __forceinline__ bool pg_elect() {
   return r != 0;
 }
 
-// A bounded wait whose answer the whole warp shares.
-__device__ __forceinline__ bool pg_warp_wait(uint32_t bar, uint32_t parity) {
-  return __all_sync(kFull, mbar_wait_bounded(bar, parity));
+// A wait of at most `polls` polls (one at least), and one whose answer the whole warp shares.
+__device__ __forceinline__ bool pg_wait(uint32_t bar, uint32_t parity, int polls) {
+#pragma unroll 1
+  for (int i = 0;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (i >= 64) __nanosleep(256);
+    if (++i >= polls) return false;
+  }
+}
+__device__ __forceinline__ bool pg_warp_wait(uint32_t bar, uint32_t parity, int polls) {
+  return __all_sync(kFull, pg_wait(bar, parity, polls));
 }
 
 template <typename T>
@@ -346,7 +356,7 @@ __device__ __forceinline__ float pg_max(const uint32_t (&r)[N]) {
 // False when a wait ran out.
 template <int D>
 __device__ __forceinline__ bool pg_reference(float mx, bool valid, bool has_o, uint32_t t_o, uint32_t b_pv,
-                                             uint32_t parity, float& mref, float& l) {
+                                             uint32_t parity, int polls, float& mref, float& l) {
   const bool need = valid && mx > mref + kPgRescale;
   if (!__any_sync(kFull, need)) return true;
   float alpha = 1.f;
@@ -356,7 +366,7 @@ __device__ __forceinline__ bool pg_reference(float mx, bool valid, bool has_o, u
     l *= alpha;
   }
   if (has_o) {
-    if (!pg_warp_wait(b_pv, parity)) return false;
+    if (!pg_warp_wait(b_pv, parity, polls)) return false;
     tc_fence_after();
 #pragma unroll 1
     for (int x = 0; x < D; x += 32) {
@@ -396,13 +406,13 @@ __device__ __forceinline__ void pg_probs(const uint32_t (&r)[N], uint64_t scale2
 template <typename T, int D, int N>
 __device__ __forceinline__ bool pg_half_step(uint32_t (&r)[N], int keys, bool valid, bool fresh, float scale,
                                              uint64_t scale2, uint32_t t_o, uint32_t b_pv, uint32_t parity,
-                                             float& mref, float& l, uint32_t* pk) {
+                                             int polls, float& mref, float& l, uint32_t* pk) {
   pg_mask(r, keys);
   uint64_t sum[2] = {0, 0};
   if (!fresh) pg_probs<T>(r, scale2, mref == kNegInf ? 0.f : mref, sum, pk);
   const float mx = pg_max(r) * scale;
   if (__any_sync(kFull, valid && mx > mref + kPgRescale) || fresh) {
-    if (!pg_reference<D>(mx, valid, !fresh, t_o, b_pv, parity, mref, l)) return false;
+    if (!pg_reference<D>(mx, valid, !fresh, t_o, b_pv, parity, polls, mref, l)) return false;
     sum[0] = sum[1] = 0;
     pg_probs<T>(r, scale2, mref == kNegInf ? 0.f : mref, sum, pk);
   }
@@ -576,6 +586,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
   }
 
   bool failed = false;
+  const int polls = A.wait_polls;
   const bool narrow_prefix = A.tiles == 1 && A.batch * A.group <= kPgNarrow;
   if (warp == kPgLoadWarp) {
     // ================================================================ loads (a lane per page of a tile)
@@ -592,6 +603,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     uint32_t phase_k = 1, phase_v = 1;         // and the parity of their release
     int tile = 0, step = 0;            // ring tiles and steps issued
     int wide = 0, thin = 0;            // wide and narrow Q tiles issued
+    int bare = 0;                      // 1: the slot after the last tile's has a phase without a copy
     // An own piece reads its rows through its own row of the table, the shared ones (the prefix's,
     // or a shorter sequence's) through row 0.  `row0`, `limit`: this lane's first row of chunk 0,
     // and where the rows end.
@@ -624,12 +636,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       }
       if (narrow && wide > 0) {  // the narrow tiles take the wide ones' place
         for (int i = wide > 1 ? wide - 2 : 0; i < wide && !failed; ++i)
-          failed = !pg_warp_wait(b_qempty + 8 * (i & 1), (i >> 1) & 1);
+          failed = !pg_warp_wait(b_qempty + 8 * (i & 1), (i >> 1) & 1, polls);
+        if (failed) break;
         wide = 0;
       }
       for (int t = 0; t < (pc.pair ? 2 : 1) && !failed; ++t) {
         const int slot = narrow ? 2 + (thin & 3) : wide & 1, use = narrow ? thin >> 2 : wide >> 1;
-        if (use > 0 && !pg_warp_wait(b_qempty + 8 * slot, (use - 1) & 1)) {
+        if (use > 0 && !pg_warp_wait(b_qempty + 8 * slot, (use - 1) & 1, polls)) {
           failed = true;
           break;
         }
@@ -649,11 +662,25 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       more = walk.next(A, L, ahead);
       if (more) rows_ahead = rows_of(ahead);
       const int first_page = more ? page_of(rows_ahead, ahead.j0) : -1;  // in flight under this piece's chunks
-      for (int j = pc.j0; j < pc.j1 && !failed; ++j) {
+      auto record = [&](int j) {  // a chunk's steps
+        const uint32_t ends = (j + 1 == pc.j1 ? PgStep::kQRelease : 0u) | (j == pc.j0 ? PgStep::kQWait : 0u);
+        if (pc.pair) {
+          const uint32_t f = ends | (j == pc.j0 ? PgStep::kFirst : 0u);
+          steps[step % kPgSteps] = f | PgStep::kMore | q_bits[0];
+          steps[(step + 1) % kPgSteps] = f | q_bits[1];
+        } else {
+          steps[step % kPgSteps] = ends | (j - pc.j0 < 2 ? PgStep::kFirst : 0u) | q_bits[0];
+        }
+      };
+      // (The test hook ends a piece early: a look at each tile made pages of 16 rows 2 % slower.)
+      const unsigned into = unsigned(A.skip_tile - tile);
+      const bool cut = into < 2u * unsigned(pc.j1 - pc.j0);
+      const int end = cut ? pc.j0 + int(into / 2) : pc.j1;
+      for (int j = pc.j0; j < end && !failed; ++j) {
         const int next_page = j + 1 < pc.j1 ? page_of(rows, j + 1) : first_page;
         const int nq = pc.pair ? 2 : 1;
-        if (kBoth && !__all_sync(kFull, mbar_wait_bounded(b_empty + 8 * slot_k, phase_k) &&
-                                            mbar_wait_bounded(b_empty + 8 * slot_v, phase_v))) {
+        if (kBoth && !__all_sync(kFull, pg_wait(b_empty + 8 * slot_k, phase_k, polls) &&
+                                            pg_wait(b_empty + 8 * slot_v, phase_v, polls))) {
           failed = true;
           break;
         }
@@ -665,22 +692,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
 #pragma unroll
         for (int v = 0; v < 2; ++v, ++tile) {
           const int r = v ? slot_v : slot_k;
-          if (!kBoth && !pg_warp_wait(b_empty + 8 * r, v ? phase_v : phase_k)) {
+          if (!kBoth && !pg_warp_wait(b_empty + 8 * r, v ? phase_v : phase_k, polls)) {
             failed = true;
             break;
           }
           const uint32_t bar = b_full + 8 * r, dst = s_ring + r * kTB + box_rows;
           if (lane == 0) {
-            if (v == 0) {  // the chunk's steps, published by the arrival
-              const uint32_t ends = (j + 1 == pc.j1 ? PgStep::kQRelease : 0u) | (j == pc.j0 ? PgStep::kQWait : 0u);
-              if (pc.pair) {
-                const uint32_t f = ends | (j == pc.j0 ? PgStep::kFirst : 0u);
-                steps[step % kPgSteps] = f | PgStep::kMore | q_bits[0];
-                steps[(step + 1) % kPgSteps] = f | q_bits[1];
-              } else {
-                steps[step % kPgSteps] = ends | (j - pc.j0 < 2 ? PgStep::kFirst : 0u) | q_bits[0];
-              }
-            }
+            if (v == 0) record(j);  // published by the arrival
             mbar_arrive_expect_tx(bar, kTB);
           }
           __syncwarp();
@@ -695,21 +713,37 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         step += nq;
         page = next_page;
       }
-    }
-    if (!failed) {  // tell the MMA warps that the steps end here
-      if (!pg_warp_wait(b_empty + 8 * slot_k, phase_k)) {
+      if (cut && !failed) {
         failed = true;
-      } else if (lane == 0) {
-        steps[step % kPgSteps] = PgStep::kStop;
-        mbar_arrive(b_full + 8 * slot_k);
+        if ((into & 1) && pg_warp_wait(b_empty + 8 * slot_k, phase_k, polls)) {
+          // the values alone are missing: the keys' slot counts as full, with what it holds
+          if (lane == 0) {
+            record(end);
+            mbar_arrive(b_full + 8 * slot_k);
+          }
+          bare = 1;
+        }
       }
     }
-    if (failed) {  // let the copies in flight land before the CTA can exit (bounded waits)
-      for (int i = tile - 1; i >= 0 && i >= tile - kRing; --i)
-        pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1);
-      for (int i = wide - 1; i >= 0 && i >= wide - 2; --i) pg_warp_wait(b_qfull + 8 * (i & 1), (i >> 1) & 1);
-      for (int i = thin - 1; i >= 0 && i >= thin - 4; --i) pg_warp_wait(b_qfull + 8 * (2 + (i & 3)), (i >> 2) & 1);
+    if (!failed) {  // tell the MMA warps that the steps end here
+      if (!pg_warp_wait(b_empty + 8 * slot_k, phase_k, polls)) {
+        failed = true;
+      } else {
+        if (lane == 0) {
+          steps[step % kPgSteps] = PgStep::kStop;
+          mbar_arrive(b_full + 8 * slot_k);
+        }
+        bare = 1;
+      }
     }
+    // Whichever warp gives up on a wait, the copies in flight land before the CTA can exit (each
+    // wait bounded; all are there at once where nothing failed).
+    for (int i = tile - 1; i >= 0 && i >= tile - kRing + bare; --i)
+      pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1, kWaitPolls);
+    for (int i = wide - 1; i >= 0 && i >= wide - 2; --i)
+      pg_warp_wait(b_qfull + 8 * (i & 1), (i >> 1) & 1, kWaitPolls);
+    for (int i = thin - 1; i >= 0 && i >= thin - 4; --i)
+      pg_warp_wait(b_qfull + 8 * (2 + (i & 3)), (i >> 2) & 1, kWaitPolls);
   } else if (warp == kPgQkWarp) {
     // ================================================================ S = Q K^T
     // The MMA warps run as whole warps and let one lane issue: their addresses and descriptors
@@ -727,7 +761,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         r -= kRing;
         phase ^= 1;
       }
-      if (!pg_warp_wait(b_full + 8 * r, phase)) {
+      if (!pg_warp_wait(b_full + 8 * r, phase, polls)) {
         failed = true;
         break;
       }
@@ -739,8 +773,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         for (int t = 0; t < many; ++t) mbar_arrive(b_rec + 8 * ((n + t) & 3));  // the P V warp may read them too
       if (rec & PgStep::kStop) break;
       if (rec & PgStep::kQWait) {
-        if (!pg_warp_wait(b_qfull + 8 * ((rec >> 8) & 15u), (rec >> 12) & 1u)) failed = true;
-        if (many == 2 && !pg_warp_wait(b_qfull + 8 * ((rec1 >> 8) & 15u), (rec1 >> 12) & 1u)) failed = true;
+        if (!pg_warp_wait(b_qfull + 8 * ((rec >> 8) & 15u), (rec >> 12) & 1u, polls)) failed = true;
+        if (many == 2 && !pg_warp_wait(b_qfull + 8 * ((rec1 >> 8) & 15u), (rec1 >> 12) & 1u, polls)) failed = true;
         if (failed) break;
       }
       const uint64_t kd = desc + ((s_ring + r * kTB) >> 4);
@@ -748,8 +782,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         // One step on the chunk: its 128 keys in one go (an MMA of 64 keys holds the tensor core as
         // long as one of 128).
         const int s = n & 1;
-        if (n >= 2 && (!pg_warp_wait(b_pv + 16 * s, ((n >> 1) - 1) & 1) ||
-                       !pg_warp_wait(b_pv + 16 * s + 8, ((n >> 1) - 1) & 1))) {
+        if (n >= 2 && (!pg_warp_wait(b_pv + 16 * s, ((n >> 1) - 1) & 1, polls) ||
+                       !pg_warp_wait(b_pv + 16 * s + 8, ((n >> 1) - 1) & 1, polls))) {
           failed = true;
           break;
         }
@@ -771,7 +805,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           for (int t = 0; t < many; ++t) {
             const int s = (n + t) & 1;
             // the buffer is free once the product of two steps ago has read its probabilities
-            if (n + t >= 2 && !pg_warp_wait(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1)) {
+            if (n + t >= 2 && !pg_warp_wait(b_pv + 8 * (2 * s + h), (((n + t) >> 1) - 1) & 1, polls)) {
               failed = true;
               break;
             }
@@ -800,7 +834,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       n += many;
     }
     if (leader) tc_commit(b_done);  // TMEM is freed only after every MMA has completed
-    pg_warp_wait(b_done, 0);
+    pg_warp_wait(b_done, 0, kWaitPolls);
   } else if (warp == kPgPvWarp) {
     // ================================================================ O += P V
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -809,15 +843,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     const bool leader = pg_elect();
     int r = 1, phase = 0;  // ring slot and phase parity of the chunk's V
     for (int n = 0;;) {
-      if (!pg_warp_wait(b_rec + 8 * (n & 3), (n >> 2) & 1)) {
+      if (!pg_warp_wait(b_rec + 8 * (n & 3), (n >> 2) & 1, polls)) {
         failed = true;
         break;
       }
       const uint32_t rec = steps[n % kPgSteps];  // a pair's two steps are alike here
       if (rec & PgStep::kStop) break;
       const int many = rec & PgStep::kMore ? 2 : 1;
-      if (many == 2 && !pg_warp_wait(b_rec + 8 * ((n + 1) & 3), ((n + 1) >> 2) & 1)) failed = true;
-      if (failed || !pg_warp_wait(b_full + 8 * r, phase)) {
+      if (many == 2 && !pg_warp_wait(b_rec + 8 * ((n + 1) & 3), ((n + 1) >> 2) & 1, polls)) failed = true;
+      if (failed || !pg_warp_wait(b_full + 8 * r, phase, polls)) {
         failed = true;
         break;
       }
@@ -828,7 +862,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
 #pragma unroll 1
         for (int t = 0; t < many; ++t) {
           const int s = (n + t) & 1;
-          if (!pg_warp_wait(b_p + 8 * (2 * s + h), ((n + t) >> 1) & 1)) {
+          if (!pg_warp_wait(b_p + 8 * (2 * s + h), ((n + t) >> 1) & 1, polls)) {
             failed = true;
             break;
           }
@@ -852,7 +886,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       n += many;
     }
     if (leader) tc_commit(b_done);
-    pg_warp_wait(b_done, 0);
+    pg_warp_wait(b_done, 0, kWaitPolls);
   } else {
     // ================================================================ softmax: warpgroup s, a thread per query row
     const int s = warp >> 2, row = tid & 127, wq = warp & 3;
@@ -866,7 +900,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
     };
     auto wg_sync = [&]() -> bool {  // the warpgroup's threads, bounded
       arrive(b_wg + 8 * s);
-      return pg_warp_wait(b_wg + 8 * s, (syncs++) & 1);
+      return pg_warp_wait(b_wg + 8 * s, (syncs++) & 1, polls);
     };
     // whether prefix row r of tile `tile` belongs to a sequence that has the whole prefix
     auto takes_part = [&](int tile, int r) { return paged_len(A, tile * A.per_tile + r / A.group) >= A.shared; };
@@ -885,7 +919,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         const int st = pc.pair ? step + 2 * c + t : step + c;
         const int limit = end - (pc.j0 + c) * kPgKeys;  // keys of this chunk that count
         const uint32_t phase = (st >> 1) & 1;
-        if (!pg_warp_wait(b_s + 16 * s, phase)) {
+        if (!pg_warp_wait(b_s + 16 * s, phase, polls)) {
           failed = true;
           break;
         }
@@ -894,7 +928,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           // probability of 0 gives 0.  (This step's scores are there, so the slot's tile before has
           // been read and the barrier is in this tile's phase.)
           const int i = 2 * (chunk + c) + 1;
-          if (!pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1)) {
+          if (!pg_warp_wait(b_full + 8 * (i % kRing), (i / kRing) & 1, polls)) {
             failed = true;
             break;
           }
@@ -907,7 +941,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           fence_proxy_async_smem();
         }
         if (narrow) {  // both halves at once: a warp's keys are in one of them
-          if (!pg_warp_wait(b_s + 16 * s + 8, phase)) {
+          if (!pg_warp_wait(b_s + 16 * s + 8, phase, polls)) {
             failed = true;
             break;
           }
@@ -917,7 +951,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
           tc_wait_ld();
           // (the product before is complete: the second half's scores were issued after it)
           if (!pg_half_step<T, D>(r, limit - 32 * wq, lane < rows, c < inc, A.scale_log2, scale2, t_o, b_pv + 16 * s + 8,
-                                  phase ^ 1, mref, l, pk)) {
+                                  phase ^ 1, polls, mref, l, pk)) {
             failed = true;
             break;
           }
@@ -938,7 +972,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
         }
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          if (h == 1 && !pg_warp_wait(b_s + 16 * s + 8, phase)) {
+          if (h == 1 && !pg_warp_wait(b_s + 16 * s + 8, phase, polls)) {
             failed = true;
             break;
           }
@@ -949,7 +983,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
             tc_wait_ld();
             // the half step before on this stream: its product is complete before O may be rescaled
             if (!pg_half_step<T, D>(r, limit - h * kPgHalf, row < rows, c < inc && h == 0, A.scale_log2, scale2, t_o,
-                                    b_pv + 16 * s + 8 * (h ^ 1), phase ^ h ^ 1, mref, l, pk)) {
+                                    b_pv + 16 * s + 8 * (h ^ 1), phase ^ h ^ 1, polls, mref, l, pk)) {
               failed = true;
               break;
             }
@@ -968,7 +1002,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) sink_paged_kernel(const __grid_
       } else if (!failed) {
         // ---- this stream's partial result of the piece
         const int st = pc.pair ? step + 2 * (n - 1) + t : step + t + (n - 1 - t) / 2 * 2;  // the last step
-        if (!pg_warp_wait(b_pv + 8 * (2 * s + 1), (st >> 1) & 1)) failed = true;
+        if (!pg_warp_wait(b_pv + 8 * (2 * s + 1), (st >> 1) & 1, polls)) failed = true;
         tc_fence_after();
         if (narrow) {
           // the four warps' results over their keys, joined in shared memory

@@ -372,8 +372,19 @@ constexpr int cluster_warps() {
 }
 
 // Failure-detection test hook (sink_debug_fail_next_wait): armed as (chunk << 32) | polls,
-// consumed by the next stream-kernel launch of the process; -1 when disarmed.
+// consumed by the next launch of the stream or the paged attention kernel in the process; -1
+// when disarmed.
 std::atomic<int64_t> g_fail_next_wait{-1};
+
+}  // namespace
+
+namespace sinkb200 {
+
+int64_t take_fail_next_wait() { return g_fail_next_wait.exchange(-1, std::memory_order_acq_rel); }
+
+}  // namespace sinkb200
+
+namespace {
 
 // Cluster placement override (sink_debug_cluster_capacity): -1 asks the device; n >= 0 is
 // taken as every clustered stream launch's capacity.
@@ -443,7 +454,7 @@ int32_t launch_stream(const StreamArgs& A0, const Plan& pl, int pairs, cudaStrea
     *capacity = cluster_capacity(kern, threads, smem, pl.ns, dev, st);
     return SINK_OK;
   }
-  const int64_t inject = g_fail_next_wait.exchange(-1, std::memory_order_acq_rel);  // launches only
+  const int64_t inject = take_fail_next_wait();  // launches only
   if (inject >= 0) {
     A.skip_chunk = int(inject >> 32);
     A.wait_polls = int(inject & 0x7fffffff);

@@ -302,7 +302,11 @@ int32_t sink_v2_decode_step(const sink_kv_buffers_t* kv, const sink_rows_t* k_ne
  * SINK_STATUS_WAIT_TIMEOUT in the workspace status word; the context stays usable.  CTAs
  * whose split has no chunk `chunk` run normally.  A launch that fails this way leaves an
  * in-place eviction partly applied, so the caller restores the buffers (a read-only
- * attention leaves them untouched).  Returns 0, or SINK_EINVAL for chunk < 0 or polls < 1.
+ * attention leaves them untouched).
+ * A launch of sink_paged_attention takes it too: `chunk` counts the tiles that a CTA copies,
+ * 2 c the 128 keys of its c-th chunk and 2 c + 1 their values; neither that tile nor those
+ * behind it are copied, the status word is the paged cache's, and the output is void.
+ * Returns 0, or SINK_EINVAL for chunk < 0 or polls < 1.
  */
 int32_t sink_debug_fail_next_wait(int32_t chunk, int32_t polls);
 
