@@ -76,8 +76,11 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, kind: str = "default",
     base ** (-2i / rot_dim), then, for contexts `factor` times the `original_length` the model
     was trained on:
       "linear"   every frequency divided by factor (positions interpolated);
-      "ntk"      the base raised so that the lowest frequency reaches a context of `length` (the
-                 original length times factor when not given);
+      "ntk"      the base multiplied by (factor * reach - (factor - 1)) ** (rot_dim / (rot_dim - 2)),
+                 reach = length / original_length, at least 1: the highest frequency stays and the
+                 lowest is divided by factor * reach - (factor - 1).  `length` is the context to be
+                 served, original_length * factor when not given (a lowest frequency divided by
+                 factor**2 - factor + 1); factor 1 divides by reach alone;
       "llama3"   wavelengths above original_length / low_freq_factor divided by factor, those
                  below original_length / high_freq_factor kept, a linear blend between;
       "yarn"     pairs that turn more than beta_fast times over the original length kept, those

@@ -244,3 +244,34 @@ def test_every_status_bit_is_reported():
         with pytest.raises(RuntimeError, match=f"sinkcache_b200.*0x{status:x}") as e:
             _lib.raise_status(status)
         assert all(x in str(e.value) for x in there) and not any(x in str(e.value) for x in absent)
+
+
+@pytest.mark.parametrize("factor,length,divisor", [(4.0, None, 13.0), (2.0, None, 3.0), (4.0, 16384, 13.0),
+                                                   (4.0, 8192, 5.0), (4.0, 4096, 1.0), (4.0, 1000, 1.0),
+                                                   (1.0, 16384, 4.0)])
+def test_ntk_frequencies_as_documented(factor, length, divisor):
+    """Highest frequency kept, lowest divided by factor * reach - (factor - 1); every frequency is the
+    same power of the raised base."""
+    f = rope_frequencies(64, 50000.0)[0]
+    ntk, scaling = rope_frequencies(64, 50000.0, "ntk", factor, original_length=4096, length=length)
+    assert scaling == 1.0 and ntk[0] == f[0]
+    torch.testing.assert_close(f[-1] / ntk[-1], torch.tensor(divisor, dtype=torch.float64))
+    torch.testing.assert_close(f / ntk, divisor ** (torch.arange(32, dtype=torch.float64) / 31))
+    torch.testing.assert_close(rope_frequencies(2, kind="ntk", factor=4.0)[0], torch.ones(1, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("kind", ["linear", "llama3", "yarn", "dynamic"])
+@pytest.mark.parametrize("length", [4096, 10000, 16384])
+def test_frequencies_match_the_model_library(kind, length):
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    params = {"rope_type": kind, "rope_theta": 50000.0, "factor": 4.0, "original_max_position_embeddings": 4096,
+              "low_freq_factor": 1.0, "high_freq_factor": 4.0}
+    c = LlamaConfig(hidden_size=1024, num_attention_heads=8, head_dim=128, max_position_embeddings=4096,
+                    rope_parameters=params)
+    want, scaling = ROPE_INIT_FUNCTIONS[kind](c, torch.device("cpu"), seq_len=length)
+    f, a = rope_frequencies(128, 50000.0, "ntk" if kind == "dynamic" else kind, 4.0, 4096, length)
+    # the library's are fp32: the exponent 2 i / 128, its power (ln 50000 = 10.8 times its rounding) and a
+    # division or blend, some 16 units of 2^-24 in all
+    torch.testing.assert_close(f, want.double(), rtol=16 * 2.0 ** -24, atol=0)
+    assert abs(a - scaling) < 1e-6
