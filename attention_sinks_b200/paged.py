@@ -171,7 +171,8 @@ class PagedKVCache:
         positions.  Returns q [B, Hq, T, D] rotated to them too, in one launch (None without q).
         Tokens from counts[b] on, and all of an idle sequence's (lens 0), are not stored; their
         q rows come back as zeros.  counts: int32 [B] on the device.  Sequences may share pages that
-        they read; of two that append to one slot, one row stays."""
+        they read, not slots that they append to: a slot that two write in one call holds each
+        value of its rows from one or the other."""
         if _lib.current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.append(k, v, q, counts)

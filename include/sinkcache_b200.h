@@ -433,8 +433,8 @@ typedef struct sink_paged_kv {
  * everywhere.  Tokens from counts[b] on, and tokens whose position is negative (an idle
  * sequence: lens 0), are not written.
  * q / q_out (both or neither; [batch, heads, n, head_dim]): rotated to the same positions in the
- * same launch, zeros for tokens that are not written.  Two sequences that append to one slot
- * leave one of the two rows there.
+ * same launch, zeros for tokens that are not written.  A slot that two sequences append to in one
+ * call holds each value of its rows from one or the other (no order between them).
  */
 int32_t sink_paged_append(const sink_paged_kv_t* kv, const sink_rows_t* k_new,
                           const sink_rows_t* v_new, const int32_t* counts, const sink_rows_t* q,

@@ -99,3 +99,22 @@ def test_sizes_past_32_bits_are_refused_not_cut():
     with pytest.raises(ValueError, match="32 bits"):
         cache.append(many, many)
     assert torch.equal(cache.v_pages.view(torch.int16), before.view(torch.int16))
+
+
+def test_two_sequences_that_append_to_one_slot():
+    """Each value of the slot is one sequence's or the other's, and nothing else moves."""
+    g = gen(47)
+    cache = make_cache(g, [40, 40, 20], 2, 16, 64, fill=0.0)
+    cache.block_table[1, 2] = cache.block_table[0, 2]
+    k, v = randn(g, 3, 2, 4, 64), randn(g, 3, 2, 4, 64)
+    before = [x.clone() for x in (cache.k_pages, cache.v_pages)]
+    cache.append(k, v)
+    cache.check_status()
+    page = int(cache.block_table[0, 2])
+    for pages, was, new in zip((cache.k_pages, cache.v_pages), before, (k, v)):
+        got = pages[page, :, 4:8]
+        assert bool(((got == new[0]) | (got == new[1])).all())
+        was[page, :, 4:8] = got
+        own = int(cache.block_table[2, 1])
+        was[own, :, 0:4] = new[2]
+        assert torch.equal(pages, was)
