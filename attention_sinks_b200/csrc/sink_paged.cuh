@@ -1194,7 +1194,8 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
       o.w += v.w;
     }
   }
-  const float total = team == 0 ? inv[g] : 0.f, r = total == 0.f ? 0.f : 1.f / total;
+  // (a sum of 0 over rows that are there is that of scores all -infinity: 0 / 0, as in the formula)
+  const float total = team == 0 ? inv[g] : 0.f, r = 1.f / total;
   float y[4] = {o.x * r, o.y * r, o.z * r, o.w * r};
   // A narrow tile meets every value with the probability 0 of the warps whose key it is not, and 0
   // times an infinity is NaN; so is it where a probability or weight that is not 0 rounds to 0.
@@ -1215,7 +1216,7 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
   if (team == 0) {
     T* out = reinterpret_cast<T*>(A.out) + b * A.o_sb + (h * G + g) * A.o_sh + 4 * x;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = Elem<T>::from_f(total == 0.f ? 0.f : y[k]);
+    for (int k = 0; k < 4; ++k) out[k] = Elem<T>::from_f(len == 0 ? 0.f : y[k]);
   }
 }
 

@@ -134,3 +134,40 @@ def test_an_infinite_value_of_small_probability(shared):
     clean = formula(cache, q, shared)
     put(cache.v_pages, cache, 0, 71, 0, -INF, dim=11, shared=shared)
     assert check(cache, q, clean, shared)[0, 0, 0, 11] == -INF
+
+
+@pytest.mark.parametrize("batch,shared,own", [(2, 0, 1), (2, 0, 130), (2, 0, 1000), (2, 128, 40), (33, 256, 20)])
+def test_scores_that_are_all_minus_infinity(batch, shared, own):
+    """A softmax over nothing but -infinity is 0 / 0, NaN; some of them alone are left out."""
+    g = gen(batch + own)
+    cache = make_cache(g, [shared + own + i for i in range(batch)], 2, 64, 128, shared=shared)
+    q = randn(g, batch, 4, 1, 128)
+    q[0, 2:, 0, 3] = 1.0
+    for pos in range(shared + own):
+        put(cache.k_pages, cache, 0, pos, 1, -INF, dim=3, shared=shared)
+    want, _ = formula(cache, q, shared)
+    got = cache.attend(q, shared_len=shared)
+    assert torch.isnan(got[0, 0, 2:]).all() and torch.isnan(want[0, 0, 2:]).all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+def test_some_scores_of_minus_infinity_count_as_nothing():
+    """Bound: that of the formula over the rows that are left."""
+    g = gen(9)
+    lens, out = [300, 200], (0, 1, 2, 5, 140, *range(160, 192), 299)
+    cache = make_cache(g, lens, 2, 64, 128)
+    q = randn(g, 2, 4, 1, 128)
+    q[0, 2:, 0, 3] = 1.0
+    left = make_cache(gen(10), [300 - len(out)], 2, 64, 128)
+    for pages, to in ((cache.k_pages, left.k_pages), (cache.v_pages, left.v_pages)):
+        rows = ref.gather(pages, cache.block_table[0], 300)
+        rows = rows[:, [p for p in range(300) if p not in out]]
+        for n in range(rows.shape[1]):
+            to[int(left.block_table[0, n // 64]), :, n % 64] = rows[:, n].to(to.dtype)
+    want, bound = formula(left, q[:1])
+    for pos in out:
+        put(cache.k_pages, cache, 0, pos, 1, -INF, dim=3)
+    got = cache.attend(q)
+    cache.check_status()
+    ref.assert_bounded(got[:1, :, 2:], want[:, :, 2:], bound[:, :, 2:])
+    assert torch.isfinite(got).all()
