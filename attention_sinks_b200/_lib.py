@@ -540,8 +540,8 @@ class RowsArg:
         if t.dim() != 4 or t.stride(-1) != 1:
             raise ValueError(f"expected a [B, H, n, D] tensor with unit last stride, got {tuple(t.shape)} "
                              f"strides {t.stride()}")
-        self.rows = Rows(0, dtype_code(t.dtype), int32("heads", t.shape[1]), int32("tokens", t.shape[2]), 0, t.stride(0),
-                         t.stride(1), t.stride(2))
+        self.rows = Rows(0, dtype_code(t.dtype), int32("heads", t.shape[1]), int32("tokens", t.shape[2]), 0,
+                         t.stride(0), t.stride(1), t.stride(2))
         self.ref = ctypes.byref(self.rows)
 
     def at(self, t: torch.Tensor):

@@ -36,10 +36,10 @@
 //
 // Measured, against the rate of a plain copy (6.5 TB/s) and of a library product (1672 TFLOP/s):
 // 64 sequences of 16K own rows, 8 kv heads, D = 64: 333 us, 6.4 TB/s; of 1K to 16K rows, D = 128:
-// 374 to 418 us, 5.6 to 6.3 TB/s.  A prefix of 32K rows for 64 sequences of 4 query heads per kv
+// 374 to 432 us, 5.4 to 6.3 TB/s.  A prefix of 32K rows for 64 sequences of 4 query heads per kv
 // head, D = 128: 49 us, 700 TFLOP/s; for 256, D = 64: 131 us, 520 TFLOP/s, bound by the
 // exponentials (53 % of the special-function rate) and the wait for the products between them.
-// 4K shared and 16 to 1020 own rows, 64 sequences: 42 us for 23 us of bytes, 8 us of it start
+// 4K shared and 16 to 1020 own rows, 64 sequences: 43 us for 23 us of bytes, 8 us of it start
 // and join.
 #pragma once
 
@@ -101,7 +101,7 @@ struct PagedArgs {
   float scale_log2;  // of |scale|
   uint32_t negate;   // scale < 0: the MMA negates Q
   int wait_polls;    // of each bounded wait (kWaitPolls unless a failure-detection test shortens it)
-  int skip_tile;     // failure-detection test hook, -1 when off: the K or V tile that no CTA loads (nor those behind it)
+  int skip_tile;     // failure-detection test hook, -1 when off: the K or V tile from which on no CTA loads
 };
 
 // ------------------------------------------------------------------ the line of work

@@ -15,7 +15,8 @@ One decode step of one layer:
     out = cache.attend(q, shared_len=prefix)      # [B, 1, Hq, D]
 
 Block table, lengths and counts are device tensors that the kernels read, so a captured CUDA
-graph of the step serves every later token.
+graph of the step serves every later token.  Its kernels read and write the cache's tensors:
+keep the cache as long as the graph.
 """
 
 import ctypes
@@ -90,11 +91,12 @@ class PagedKVCache:
     """One layer's paged cache over tensors of the caller's.
 
     k_pages, v_pages: [pages, Hkv, page_size, D] pools (rows contiguous, page and head strides
-    free), bfloat16, float16 or float32.  block_table: int32 [B, width]; row p of sequence b is
-    slot p % page_size of page block_table[b, p // page_size].  lens: int32 [B], the rows of each
-    sequence, this step's tokens included; 0 for an idle sequence.  Both are read by the kernels
-    when they run: update them in place.  Layers of one model share them, and may share `status`
-    (a device int32 word that failures are recorded in).
+    free), bfloat16, float16 or float32 (`attend` takes fewer forms than `append`: it says
+    which).  block_table: int32 [B, width]; row p of sequence b is slot p % page_size of page
+    block_table[b, p // page_size].  lens: int32 [B], the rows of each sequence, this step's
+    tokens included; 0 for an idle sequence.  Both are read by the kernels when they run: update
+    them in place.  Layers of one model share them, and may share `status` (a device int32 word
+    that failures are recorded in).
 
     inv_freq (or None: keys and queries are stored and returned as they are), interleaved and
     attention_scaling are `rotary`'s.
@@ -148,8 +150,8 @@ class PagedKVCache:
     # are what keeps it: they can be updated in place (`cache.lens += 1` too) and not replaced.
     def __setattr__(self, name: str, value) -> None:
         if name in self._fixed and value is not getattr(self, name):
-            raise AttributeError(f"{name} of a paged cache cannot be replaced: update it in place, or make another cache "
-                                 "over the new one")
+            raise AttributeError(f"{name} of a paged cache cannot be replaced: update it in place, or make another "
+                                 "cache over the new one")
         super().__setattr__(name, value)
 
     def __delattr__(self, name: str) -> None:
@@ -200,7 +202,7 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, scale: float | None = None, shared_len: int = 0) -> torch.Tensor:
         """Attention of one query token per sequence, q [B, Hq, 1, D], over its rows
         [0, lens[b]): [B, 1, Hq, D] in q's type, zeros for an idle sequence.  `scale` defaults
-        to D ** -0.5.
+        to D ** -0.5.  What is not finite comes out as the formula has it.
 
         The first `shared_len` rows (a multiple of the page size) are the same for all
         sequences: they are read through the first row of the block table, once per kv head

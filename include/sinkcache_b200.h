@@ -390,8 +390,8 @@ typedef struct sink_rotation {
  * unit last stride and any other strides (0 included, for a source); q and k may differ in
  * heads; k and k_out may both be NULL.  A destination may be its own source, element for
  * element.  positions: device int64, of token t of sequence b at [b * positions_stride_b + t]
- * (stride 0 shares one row).  head_dim <= 512; fp32, bf16 or fp16; fp32 arithmetic, one
- * rounding to the type.
+ * (stride 0 shares one row).  head_dim <= 512, batch * n < 2^31; fp32, bf16 or fp16; fp32
+ * arithmetic, one rounding to the type.
  */
 int32_t sink_rotary(int32_t batch, int32_t head_dim, const sink_rows_t* q, const sink_rows_t* q_out,
                     const sink_rows_t* k, const sink_rows_t* k_out, const int64_t* positions,
@@ -430,8 +430,8 @@ typedef struct sink_paged_kv {
  * Append: the first counts[b] tokens of k_new / v_new [batch, heads_kv, n, head_dim] become rows
  * lens[b] - counts[b] .. lens[b] - 1 of sequence b, k rotated to its position on the way (rot
  * NULL: as it is).  counts: device int32 [batch] (more than n counts as n), NULL for n
- * everywhere.  Tokens from counts[b] on, and tokens whose position is negative (an idle
- * sequence: lens 0), are not written.
+ * everywhere; batch * n < 2^31.  Tokens from counts[b] on, and tokens whose position is negative
+ * (an idle sequence: lens 0), are not written.
  * q / q_out (both or neither; [batch, heads, n, head_dim]): rotated to the same positions in the
  * same launch, zeros for tokens that are not written.  A slot that two sequences append to in one
  * call holds each value of its rows from one or the other (no order between them).
@@ -449,7 +449,8 @@ size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads
 
 /*
  * Decode attention of one query token per sequence over its rows [0, lens[b]):
- *   out[b, 0, hq, :] = softmax(q[b, hq] . K^T * scale) @ V,   zeros where lens[b] <= 0.
+ *   out[b, 0, hq, :] = softmax(q[b, hq] . K^T * scale) @ V,   zeros where lens[b] <= 0,
+ * NaN and infinities as that formula has them.
  * The rows [0, shared_len) are the same for every sequence: they are read through
  * table[0] (whatever the other rows of the table hold there), once per kv head for all
  * queries; a sequence of fewer rows attends to its own number of them.  shared_len is a
