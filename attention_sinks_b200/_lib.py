@@ -281,9 +281,9 @@ class Workspace:
 
 def fail_next_wait(chunk: int, polls: int) -> None:
     """Failure-detection test hook (sink_debug_fail_next_wait): the next stream-kernel launch
-    leaves chunk `chunk` of every split unissued (the next paged attention: copy `chunk` of each
-    CTA, keys and values of its chunks in turn), with every wait bounded by `polls` polls, so that
-    wait runs out and the launch reports SINK_STATUS_WAIT_TIMEOUT."""
+    leaves chunk `chunk` of every split unissued (the next paged attention: the tiles of each CTA
+    from `chunk` on, keys and values of its chunks in turn), with every wait bounded by `polls`
+    polls, so that wait runs out and the launch reports SINK_STATUS_WAIT_TIMEOUT."""
     _check(lib().sink_debug_fail_next_wait(int(chunk), int(polls)), "sink_debug_fail_next_wait")
 
 

@@ -1200,7 +1200,8 @@ __global__ void __launch_bounds__(kPgCombineThreads) sink_paged_combine_kernel(c
   // A narrow tile meets every value with the probability 0 of the warps whose key it is not, and 0
   // times an infinity is NaN; so is it where a probability or weight that is not 0 rounds to 0.
   // Where the sum of probabilities is a number, a NaN is taken back to what the values say: the
-  // infinity that is there, if it is of one sign and no NaN beside it.
+  // infinity that is there, if it is of one sign and no NaN beside it (of a row whose score is
+  // -infinity too: its probability of exactly 0 is not told from one that rounds to 0).
   const bool odd = total != 0.f && total == total && (y[0] != y[0] || y[1] != y[1] || y[2] != y[2] || y[3] != y[3]);
   for (unsigned left = __ballot_sync(kFull, odd); left != 0; left &= left - 1) {
     const int src = __ffs(left) - 1;

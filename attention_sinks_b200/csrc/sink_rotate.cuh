@@ -12,9 +12,10 @@
 // rotation itself in fp32, and the result is rounded once to the tensor's type.
 //
 // Bound: memory (every element read once and written once).  q and k of 4 x 8192 tokens, 40
-// heads of 64, bf16: 57 to 61 us, 5.5 to 5.9 TB/s, 0.84 to 0.90 of a plain copy's rate, issue slots 67 % busy (three
-// rows in flight per thread 63 us, five CTAs per SM 76 us, streaming cache hints within 1 %); a
-// ragged append of 8 x 4096 tokens, 48 heads of 64: 52 us; one token: 3.5 us.
+// heads of 64, bf16: 57 to 61 us, 5.5 to 5.9 TB/s, 0.84 to 0.90 of a plain copy's rate, issue
+// slots 67 % busy (three rows in flight per thread 63 us, five CTAs per SM 76 us, streaming cache
+// hints within 1 %); a ragged append of 8 x 4096 tokens, 48 heads of 64: 51 to 52 us; one token:
+// 3 us.
 #pragma once
 
 #include "sink_common.cuh"

@@ -450,7 +450,8 @@ size_t sink_paged_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t heads
 /*
  * Decode attention of one query token per sequence over its rows [0, lens[b]):
  *   out[b, 0, hq, :] = softmax(q[b, hq] . K^T * scale) @ V,   zeros where lens[b] <= 0,
- * NaN and infinities as that formula has them.
+ * NaN and infinities as that formula has them (but for a row with a score of -infinity and an
+ * infinite value: the infinity, not NaN).
  * The rows [0, shared_len) are the same for every sequence: they are read through
  * table[0] (whatever the other rows of the table hold there), once per kv head for all
  * queries; a sequence of fewer rows attends to its own number of them.  shared_len is a
